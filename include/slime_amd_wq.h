@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define WQ_ABI_VERSION 18
+#define WQ_ABI_VERSION 19
 
 enum {
     WQ_OK = 0,
@@ -469,6 +469,92 @@ typedef struct wq_xxh3_desc {
 } wq_xxh3_desc;
 int wq_xxh3_128_grouped(const wq_xxh3_desc *descs, const int64_t *item_start, int n_desc, int64_t total_items,
                         void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * What lies between a backward pass and the quantisers, over many tensors: the global gradient norm, clipping by it and
+ * the AdamW update that folds the clip in and writes the low-precision weight (the tensors a weight sync then quantises).
+ *
+ * Gradients are bf16, fp16 or fp32 (any alignment that their elements have), every tensor a flat run of n elements.  The
+ * launches read one descriptor per piece of at most WQ_GRAD_ITEM elements, made from per-tensor descriptors on the device
+ * by wq_grad_make_items; the *_few forms take up to WQ_GRAD_FEW_MAX per-tensor descriptors from the HOST instead (read before
+ * the call returns).  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
+ * call and neither overflow nor lose small gradients (fp32 squares exactly).
+ *
+ * grad_scale (an inverse loss scale, 1 / number of tokens ...) multiplies every gradient; if grad_scale_dev is not NULL the
+ * factor is grad_scale * grad_scale_dev[0], read on the device.  A norm is that of the scaled gradients.
+ * coefficient = grad_scale * min(1, max_norm / (norm + 1e-6)), in fp32; a NaN norm makes it NaN, an infinite one 0 (NaN for
+ * infinite max_norm), as torch.nn.utils.clip_grads_with_norm_ has it. */
+#define WQ_GRAD_ITEM 16384
+#define WQ_GRAD_FEW_MAX 64
+enum { WQ_NORM_2 = 0, WQ_NORM_INF = 1 };
+
+typedef struct wq_grad_desc {
+    const void *g;
+    void *out;          /* clipped gradient; may be g itself (same dtype then); not read by the norms */
+    int64_t n;
+    int32_t g_dtype;    /* WQ_DTYPE_BF16, WQ_DTYPE_F16 or WQ_DTYPE_F32 */
+    int32_t out_dtype;
+} wq_grad_desc;
+
+/* starts with the fields of wq_grad_desc: `out` is the low-precision copy of the weight (NULL: none is written) */
+typedef struct wq_adamw_desc {
+    const void *g;
+    void *out;
+    int64_t n;
+    int32_t g_dtype;
+    int32_t out_dtype;
+    float *p;           /* fp32 weight */
+    float *m;           /* fp32 first and second moments */
+    float *v;
+    float lr_scale;     /* multiplies the learning rate for this tensor */
+    float weight_decay;
+} wq_adamw_desc;
+
+/* `descs`: DEVICE array of n_desc wq_grad_desc (words = 4) or wq_adamw_desc (words = 8); item_start: DEVICE int64[n_desc+1],
+ * exclusive prefix sum of ceil(n / WQ_GRAD_ITEM); items: DEVICE, n_items = item_start[n_desc] descriptors of the same kind. */
+int wq_grad_make_items(const void *descs, const int64_t *item_start, int n_desc, int64_t n_items, int words, void *items,
+                       void *stream);
+
+/* Bytes of the `workspace` (16-byte aligned, need not be cleared) of the calls below for n_items pieces; calls that share one
+ * must be ordered.  0 for n_items < 0. */
+int64_t wq_grad_workspace_bytes(int64_t n_items);
+
+/* total: fp32, the norm over all tensors.  each: NULL or fp32[n_desc], the norm of every tensor (item_start as above; it is
+ * not read without `each`).  `words` as in wq_grad_make_items. */
+int wq_grad_norm_items(const void *items, int64_t n_items, int words, const int64_t *item_start, int n_desc, int norm,
+                       float grad_scale, const float *grad_scale_dev, void *workspace, float *total, float *each, void *stream);
+int wq_grad_norm_few(const wq_grad_desc *descs, int n_desc, int norm, float grad_scale, void *workspace, float *total,
+                     void *stream);
+
+/* out = round(g * coefficient).  With total_given NULL the norm is computed first and written to `total`; otherwise
+ * total_given[0] is taken for it (a norm that was reduced over ranks) and workspace and total are not used.  Where a
+ * coefficient of exactly 1 leaves a tensor as it is (out == g), it is not rewritten.  The output ranges of different
+ * descriptors must not overlap each other or other descriptors' gradients. */
+int wq_grad_clip_items(const wq_grad_desc *items, int64_t n_items, int norm, float max_norm, float grad_scale,
+                       const float *grad_scale_dev, const float *total_given, void *workspace, float *total, void *stream);
+int wq_grad_clip_few(const wq_grad_desc *descs, int n_desc, int norm, float max_norm, float grad_scale,
+                     const float *total_given, void *workspace, float *total, void *stream);
+
+/* One AdamW step (decoupled weight decay), all arithmetic in fp32 from fp32 state, t = step + 1, g' = coefficient * g:
+ *   p1 = p - lr * lr_scale * weight_decay * p;  m = b1 * m + (1 - b1) * g';  v = b2 * v + (1 - b2) * g'^2
+ *   p  = p1 - lr * lr_scale / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  out = round(p)
+ * step: DEVICE int64, incremented by the call, so a recorded call counts its replays.  lr: host value, times lr_dev[0] if
+ * lr_dev is not NULL.  max_norm < 0: no clip (coefficient = grad_scale).  The norm is computed if it is needed (max_norm >= 0
+ * or skip_nonfinite) and total_given is NULL.  skip_nonfinite: with an infinite or NaN norm nothing is written, `step`
+ * included.  total: fp32, where a computed norm goes (NULL allowed if none is). */
+typedef struct wq_adamw_hyper {
+    double beta1, beta2, eps, lr;
+    const float *lr_dev;
+    const float *grad_scale_dev;
+    const float *total_given;
+    float *total;
+    int64_t *step;
+    float grad_scale;
+    float max_norm;
+    int32_t norm;
+    int32_t skip_nonfinite;
+} wq_adamw_hyper;
+int wq_adamw_items(const wq_adamw_desc *items, int64_t n_items, const wq_adamw_hyper *hyper, void *workspace, void *stream);
 
 #ifdef __cplusplus
 }

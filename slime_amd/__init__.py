@@ -2,7 +2,8 @@
 
 bf16 -> block-FP8 (e4m3fn, 128x128 blocks, fp32 ``weight_scale_inv``), bf16 -> group-wise INT4
 (``weight_packed`` / ``weight_scale`` / ``weight_shape``) and block-FP8 -> bf16, behind the reference's
-own function names.  Everything computes in hand-written gfx950 HIP kernels reached through the C ABI
+own function names - and, for the training step before a weight sync, the gradient norm, clip and AdamW update over
+many tensors.  Everything computes in hand-written gfx950 HIP kernels reached through the C ABI
 of ``slime_amd/lib/libslime_amd_wq.so``; there is no CPU or pure-torch fallback.
 """
 
@@ -39,6 +40,7 @@ from .int4 import (
     pack_to_int32,
     quantize,
 )
+from .optim import AdamWPlan, GradClipPlan, GradNormPlan, clip_grad_norm_, clip_grads_with_norm_, get_total_norm
 from .processors import (
     _quantize_param,
     quantize_params,
@@ -62,4 +64,5 @@ __all__ = [
     "pack_layer", "pack_to_int32",
     "quant_fp8", "quantize", "quantize_params", "quantize_params_compressed_tensors", "quantize_params_fp8",
     "quantize_weight", "tensor_fp8", "weight_dequant", "weight_dequant_bf16_scale", "_quantize_param",
+    "AdamWPlan", "GradClipPlan", "GradNormPlan", "clip_grad_norm_", "clip_grads_with_norm_", "get_total_norm",
 ]

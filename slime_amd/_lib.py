@@ -15,7 +15,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libslime_amd_wq.so")
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 # selectors (mirrors of the header's enums)
 DTYPE_BF16, DTYPE_F32, DTYPE_F16, DTYPE_F64 = 0, 1, 2, 3
@@ -27,8 +27,20 @@ INT4_GROUPS_PER_WG = 64
 INT4_DEQ_WORDS_PER_ITEM = 512
 BUCKET_COPY_MARK, BUCKET_COPY_BYTES = -1, 32768
 FP8_FEW_MAX = 4
+NORM_2, NORM_INF = 0, 1
+GRAD_ITEM, GRAD_FEW_MAX = 16384, 64
 
 _i64, _int, _vp, _u32, _u64 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
+_f32, _f64 = ctypes.c_float, ctypes.c_double
+
+
+class AdamWHyper(ctypes.Structure):
+    """wq_adamw_hyper"""
+
+    _fields_ = [("beta1", _f64), ("beta2", _f64), ("eps", _f64), ("lr", _f64), ("lr_dev", _vp), ("grad_scale_dev", _vp),
+                ("total_given", _vp), ("total", _vp), ("step", _vp), ("grad_scale", _f32), ("max_norm", _f32),
+                ("norm", ctypes.c_int32), ("skip_nonfinite", ctypes.c_int32)]
+
 
 # name -> argtypes; every symbol the header declares is listed here and resolved at load time
 SIGNATURES = {
@@ -71,6 +83,13 @@ SIGNATURES = {
     "wq_delta_overwrite_encode": [_vp, _vp, _i64, _vp, ctypes.c_uint32, _vp, _int, _vp],
     "wq_delta_xor_noalloc": [_vp, _vp, _vp, _i64, _int, _vp, _vp],
     "wq_delta_xor_grouped": [_vp, _vp, _int, _i64, _int, _int, _int, _vp],
+    "wq_grad_make_items": [_vp, _vp, _int, _i64, _int, _vp, _vp],
+    "wq_grad_workspace_bytes": [_i64],
+    "wq_grad_norm_items": [_vp, _i64, _int, _vp, _int, _int, _f32, _vp, _vp, _vp, _vp, _vp],
+    "wq_grad_norm_few": [_vp, _int, _int, _f32, _vp, _vp, _vp],
+    "wq_grad_clip_items": [_vp, _i64, _int, _f32, _f32, _vp, _vp, _vp, _vp, _vp],
+    "wq_grad_clip_few": [_vp, _int, _int, _f32, _f32, _vp, _vp, _vp, _vp],
+    "wq_adamw_items": [_vp, _i64, ctypes.POINTER(AdamWHyper), _vp, _vp],
     "wq_delta_xor_xxh3": [_vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp],
 }
 
@@ -102,7 +121,7 @@ def load() -> ctypes.CDLL:
                 raise WqLibraryError(f"{LIB_PATH} does not export {name}; rebuild the library") from exc
             fn.argtypes = argtypes
             fn.restype = (ctypes.c_char_p if name == "wq_error_string"
-                          else _i64 if name in ("wq_delta_workspace_bytes", "wq_xxh3_workspace_bytes") else _int)
+                          else _i64 if name.endswith("_workspace_bytes") else _int)
         if lib.wq_abi_version() != ABI_VERSION:
             raise WqLibraryError(f"ABI mismatch: library {lib.wq_abi_version()}, binding {ABI_VERSION}; rebuild")
         _lib = lib

@@ -1,0 +1,185 @@
+// One AdamW step over many tensors for gfx950: fp32 weights and moments, gradients in bf16, fp16 or fp32, the clip folded
+// in, and the bf16 / fp16 copy of the new weight - what a weight sync quantises - written by the same pass.
+//
+//   t = step + 1, g' = c g, p1 = p (1 - lr l w), m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2
+//   p = p1 - lr l / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), out = round(p)
+//
+// Bound by HBM: 24 bytes of state and 2 or 4 of gradient per element, plus 2 for the copy.  The step number lives on the
+// device and one workgroup works out the step's scalars (bias corrections in 64 bits), so a recorded step replays with
+// the right ones.
+
+#include "wq_grad_common.h"
+
+namespace wq {
+
+constexpr int kAdamPiecesPerXcdRun = 32;
+
+struct AdamControl {       // at the start of the workspace, written anew by every step
+    float coefficient;
+    float lr;
+    float step_size;       // lr / (1 - b1^t)
+    float inv_sqrt_bc2;    // 1 / sqrt(1 - b2^t)
+    int32_t skip;
+};
+static_assert(sizeof(AdamControl) <= kGradControlBytes, "workspace layout");
+
+struct AdamBeginArgs {
+    const char* partials;
+    int64_t n_partials;
+    double beta1, beta2, lr;
+    const float* lr_dev;
+    const float* grad_scale_dev;
+    const float* total_given;
+    float* total;
+    int64_t* step;
+    float grad_scale, max_norm;
+    int32_t need_norm, skip_nonfinite;
+};
+
+template <int NORM>
+__global__ __launch_bounds__(1024) void adamw_begin_kernel(const AdamBeginArgs a, AdamControl* control)
+{
+    typedef typename NormAcc<NORM>::T T;
+    __shared__ T lds[16];
+    const float scale = effective_scale(a.grad_scale, a.grad_scale_dev);
+    float norm = 0.0f;
+    if (a.need_norm) {
+        if (a.total_given) norm = ldg<float>(a.total_given);
+        else norm = NormAcc<NORM>::finish(fold_partials<NORM>(a.partials, a.n_partials, lds), scale);
+    }
+    if (threadIdx.x) return;
+    if (a.need_norm && !a.total_given) stg<float>(a.total, norm);
+    AdamControl c;
+    c.coefficient = a.max_norm >= 0.0f ? clip_coefficient(norm, a.max_norm, scale) : scale;
+    c.skip = a.skip_nonfinite && !(norm <= 3.4028234663852886e38f);
+    const int64_t t = ldg<int64_t>(a.step) + 1;
+    const double lr = a.lr_dev ? a.lr * (double)ldg<float>(a.lr_dev) : a.lr;
+    c.lr = (float)lr;
+    c.step_size = (float)(lr / (1.0 - pow(a.beta1, (double)t)));
+    c.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+    WQ_GLOBAL AdamControl* out = (WQ_GLOBAL AdamControl*)control;
+    out->coefficient = c.coefficient;
+    out->lr = c.lr;
+    out->step_size = c.step_size;
+    out->inv_sqrt_bc2 = c.inv_sqrt_bc2;
+    out->skip = c.skip;
+    if (!c.skip) stg<int64_t>(a.step, t);
+}
+
+struct AdamConsts {
+    float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
+};
+struct AdamStep {          // the constants of a piece
+    float c, decay, step_size, inv_sqrt_bc2;
+};
+
+__device__ __forceinline__ void adam_elem(float g, float& p, float& m, float& v, const AdamConsts& k, const AdamStep& s)
+{
+    g *= s.c;
+    m = __builtin_fmaf(k.one_minus_beta1, g, k.beta1 * m);
+    v = __builtin_fmaf(k.one_minus_beta2 * g, g, k.beta2 * v);
+    const float denom = __builtin_fmaf(__builtin_sqrtf(v), s.inv_sqrt_bc2, k.eps);
+    p = __builtin_fmaf(-s.step_size, m / denom, __builtin_fmaf(-s.decay, p, p));
+}
+
+template <int G, int O>     // O < 0: no copy
+__device__ __forceinline__ void adam_piece(const wq_adamw_desc& d, const AdamConsts& k, const AdamStep& s)
+{
+    const char* g = (const char*)d.g;
+    char *p = (char*)d.p, *m = (char*)d.m, *v = (char*)d.v, *o = (char*)d.out;
+    const int n = (int)d.n, whole = n / 4;
+    for (int i = threadIdx.x; i < whole; i += kGradThreads) {
+        float gf[4];
+        if constexpr (G == WQ_DTYPE_F32) {
+            const u32x4 w = ldg16(g + (size_t)i * 16);
+            gf[0] = u2f(w.x), gf[1] = u2f(w.y), gf[2] = u2f(w.z), gf[3] = u2f(w.w);
+        } else {
+            const u32x2 w = ldg8(g + (size_t)i * 8);
+            const f32x2 a = unpack2<G>(w.x), b = unpack2<G>(w.y);
+            gf[0] = a.x, gf[1] = a.y, gf[2] = b.x, gf[3] = b.y;
+        }
+        u32x4 pw = ldg16(p + (size_t)i * 16), mw = ldg16(m + (size_t)i * 16), vw = ldg16(v + (size_t)i * 16);
+        float pf[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float mf = u2f(mw[e]), vf = u2f(vw[e]);
+            pf[e] = u2f(pw[e]);
+            adam_elem(gf[e], pf[e], mf, vf, k, s);
+            pw[e] = f2u(pf[e]), mw[e] = f2u(mf), vw[e] = f2u(vf);
+        }
+        stg16(p + (size_t)i * 16, pw);
+        stg16(m + (size_t)i * 16, mw);
+        stg16(v + (size_t)i * 16, vw);
+        if constexpr (O >= 0) stg8(o + (size_t)i * 8, (u32x2){pack2<O>(pf[0], pf[1]), pack2<O>(pf[2], pf[3])});
+    }
+    const int e = whole * 4 + threadIdx.x;
+    if (e < n) {
+        float pf = ldg<float>(p + (size_t)e * 4), mf = ldg<float>(m + (size_t)e * 4), vf = ldg<float>(v + (size_t)e * 4);
+        adam_elem(load_elem<G>(g, e), pf, mf, vf, k, s);
+        stg<float>(p + (size_t)e * 4, pf);
+        stg<float>(m + (size_t)e * 4, mf);
+        stg<float>(v + (size_t)e * 4, vf);
+        if constexpr (O >= 0) store_elem<O>(o, e, pf);
+    }
+}
+template <int G>
+__device__ __forceinline__ void adam_piece_from(const wq_adamw_desc& d, const AdamConsts& k, const AdamStep& s)
+{
+    if (!d.out) adam_piece<G, -1>(d, k, s);
+    else if (d.out_dtype == WQ_DTYPE_BF16) adam_piece<G, WQ_DTYPE_BF16>(d, k, s);
+    else adam_piece<G, WQ_DTYPE_F16>(d, k, s);
+}
+
+__global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc* items, const int64_t n_items, const AdamConsts k,
+                                                            const AdamControl* control)
+{
+    const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    if (slot >= n_items) return;  // uniform per workgroup
+    const AdamControl c = *control;
+    if (c.skip) return;
+    const wq_adamw_desc d = items[xcd_chunked_item(slot, n_items, kAdamPiecesPerXcdRun)];
+    const AdamStep s = {c.coefficient, c.lr * d.lr_scale * d.weight_decay, c.step_size * d.lr_scale, c.inv_sqrt_bc2};
+    if (d.g_dtype == WQ_DTYPE_BF16) adam_piece_from<WQ_DTYPE_BF16>(d, k, s);
+    else if (d.g_dtype == WQ_DTYPE_F16) adam_piece_from<WQ_DTYPE_F16>(d, k, s);
+    else adam_piece_from<WQ_DTYPE_F32>(d, k, s);
+}
+
+}  // namespace wq
+
+using namespace wq;
+
+WQ_EXPORT int wq_adamw_items(const wq_adamw_desc* items, int64_t n_items, const wq_adamw_hyper* h, void* workspace, void* stream)
+{
+    if (n_items < 0) return WQ_ERR_SHAPE;
+    if (!h || !workspace || !h->step || (n_items && !items)) return WQ_ERR_NULL;
+    if (h->norm != WQ_NORM_2 && h->norm != WQ_NORM_INF) return WQ_ERR_MODE;
+    if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0)) return WQ_ERR_SHAPE;
+    const bool need_norm = h->max_norm >= 0.0f || h->skip_nonfinite;
+    if (need_norm && !h->total_given && !h->total) return WQ_ERR_NULL;
+    hipStream_t st = (hipStream_t)stream;
+    AdamBeginArgs a = {};
+    a.partials = partials_of(workspace);
+    a.n_partials = n_items;
+    a.beta1 = h->beta1;
+    a.beta2 = h->beta2;
+    a.lr = h->lr;
+    a.lr_dev = h->lr_dev;
+    a.grad_scale_dev = h->grad_scale_dev;
+    a.total_given = h->total_given;
+    a.total = h->total;
+    a.step = h->step;
+    a.grad_scale = h->grad_scale;
+    a.max_norm = h->max_norm;
+    a.need_norm = need_norm;
+    a.skip_nonfinite = h->skip_nonfinite;
+    if (need_norm && !h->total_given) launch_norm_partials(TableSource{(const int64_t*)items, 8}, n_items, h->norm, partials_of(workspace), st);
+    AdamControl* control = (AdamControl*)workspace;
+    if (h->norm == WQ_NORM_2) adamw_begin_kernel<WQ_NORM_2><<<1, 1024, 0, st>>>(a, control);
+    else adamw_begin_kernel<WQ_NORM_INF><<<1, 1024, 0, st>>>(a, control);
+    if (n_items) {
+        const AdamConsts k = {(float)h->beta1, (float)(1.0 - h->beta1), (float)h->beta2, (float)(1.0 - h->beta2), (float)h->eps};
+        adamw_kernel<<<grid_for_items(n_items), kGradThreads, 0, st>>>(items, n_items, k, control);
+    }
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}

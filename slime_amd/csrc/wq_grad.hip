@@ -1,0 +1,310 @@
+// The global gradient norm over many tensors and clipping by it, for gfx950.
+//
+//   norm_2 = s * sqrt(sum g^2), norm_inf = s * max |g|, coefficient = s * min(1, max_norm / (norm + 1e-6)), out = round(g * c)
+//
+// Both are bound by HBM: the norm reads every gradient once, the clip reads it again and writes it.  One workgroup takes one
+// piece of at most 16384 elements of one tensor and leaves one 64-bit partial; a fold of the partials in a fixed order
+// gives the norm (no atomics, so the same gradients give the same bits).  Squares are added in 64 bits: fp32 squares are
+// exact there and can neither overflow nor vanish.
+
+#include "wq_grad_common.h"
+
+namespace wq {
+
+constexpr int kNormPiecesPerXcdRun = 32;
+
+// ---- norm of a piece ------------------------------------------------------------------------------------------------
+template <int NORM, int D>
+__device__ __forceinline__ void add_vec(typename NormAcc<NORM>::T& a, u32x4 v)
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (D == WQ_DTYPE_F32) {
+            NormAcc<NORM>::add(a, u2f(v[k]));
+        } else {
+            const f32x2 f = unpack2<D>(v[k]);
+            NormAcc<NORM>::add(a, f.x);
+            NormAcc<NORM>::add(a, f.y);
+        }
+    }
+}
+template <int NORM, int D>
+__device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece& p)
+{
+    constexpr int kVec = 16 / dtype_bytes(D), kLoads = 8;
+    typename NormAcc<NORM>::T a = NormAcc<NORM>::zero();
+    const int t = threadIdx.x;
+    if (p.n == kGradItem) {
+#pragma unroll
+        for (int b = 0; b < kGradItem / (kVec * kGradThreads * kLoads); ++b) {
+            u32x4 v[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i] = ldg16(p.g + (size_t)((b * kLoads + i) * kGradThreads + t) * 16);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) add_vec<NORM, D>(a, v[i]);
+        }
+    } else {
+        const int whole = p.n / kVec;
+        for (int i = t; i < whole; i += kGradThreads) add_vec<NORM, D>(a, ldg16(p.g + (size_t)i * 16));
+        const int e = whole * kVec + t;
+        if (e < p.n) NormAcc<NORM>::add(a, load_elem<D>(p.g, e));
+    }
+    return a;
+}
+
+template <int NORM, typename Source>
+__global__ __launch_bounds__(kGradThreads) void grad_norm_partials_kernel(const Source src, const int64_t n_items, char* partials)
+{
+    typedef typename NormAcc<NORM>::T T;
+    __shared__ T lds[kGradThreads / 64];
+    const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    if (slot >= n_items) return;  // uniform per workgroup
+    const int64_t item = xcd_chunked_item(slot, n_items, kNormPiecesPerXcdRun);
+    const GradPiece p = src.piece(item);
+    T a;
+    if (p.g_dtype == WQ_DTYPE_BF16) a = piece_norm<NORM, WQ_DTYPE_BF16>(p);
+    else if (p.g_dtype == WQ_DTYPE_F16) a = piece_norm<NORM, WQ_DTYPE_F16>(p);
+    else a = piece_norm<NORM, WQ_DTYPE_F32>(p);
+    a = block_fold<NORM, kGradThreads / 64>(a, lds);
+    if (threadIdx.x == 0) stg<T>(partials + item * 8, a);
+}
+
+template <int NORM>
+__global__ __launch_bounds__(1024) void grad_norm_total_kernel(const char* partials, const int64_t n, const float scale,
+                                                              const float* scale_dev, float* total)
+{
+    typedef typename NormAcc<NORM>::T T;
+    __shared__ T lds[16];
+    const T a = fold_partials<NORM>(partials, n, lds);
+    if (threadIdx.x == 0) stg<float>(total, NormAcc<NORM>::finish(a, effective_scale(scale, scale_dev)));
+}
+
+// one wavefront per tensor
+template <int NORM>
+__global__ __launch_bounds__(64) void grad_norm_each_kernel(const char* partials, const int64_t* item_start, const float scale,
+                                                           const float* scale_dev, float* each)
+{
+    typedef typename NormAcc<NORM>::T T;
+    const int64_t from = item_start[blockIdx.x], to = item_start[blockIdx.x + 1];
+    T a = NormAcc<NORM>::zero();
+    for (int64_t i = from + threadIdx.x; i < to; i += 64) a = NormAcc<NORM>::join(a, ldg<T>(partials + i * 8));
+    a = wave_fold<NORM>(a);
+    if (threadIdx.x == 0) stg<float>(each + blockIdx.x, NormAcc<NORM>::finish(a, effective_scale(scale, scale_dev)));
+}
+
+// ---- clip of a piece --------------------------------------------------------------------------------------------------
+// A lane takes the elements of one 16-byte access of the wider of the two types.
+template <int G, int O>
+__device__ __forceinline__ void piece_scale(const GradPiece& p, float c)
+{
+    constexpr bool kWide = G == WQ_DTYPE_F32 || O == WQ_DTYPE_F32;
+    constexpr int kElems = kWide ? 4 : 8;
+    const int whole = p.n / kElems;
+    for (int i = threadIdx.x; i < whole; i += kGradThreads) {
+        float f[kElems];
+        if constexpr (G == WQ_DTYPE_F32) {
+            const u32x4 v = ldg16(p.g + (size_t)i * 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = u2f(v[k]) * c;
+        } else {
+            uint32_t w[kElems / 2];
+            if constexpr (kElems == 8) {
+                const u32x4 v = ldg16(p.g + (size_t)i * 16);
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            } else {
+                const u32x2 v = ldg8(p.g + (size_t)i * 8);
+                w[0] = v.x, w[1] = v.y;
+            }
+#pragma unroll
+            for (int k = 0; k < kElems / 2; ++k) {
+                const f32x2 x = unpack2<G>(w[k]);
+                f[2 * k] = x.x * c;
+                f[2 * k + 1] = x.y * c;
+            }
+        }
+        if constexpr (O == WQ_DTYPE_F32) {
+            stg16(p.out + (size_t)i * 16, (u32x4){f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])});
+        } else if constexpr (kElems == 8) {
+            stg16(p.out + (size_t)i * 16, (u32x4){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3]), pack2<O>(f[4], f[5]), pack2<O>(f[6], f[7])});
+        } else {
+            stg8(p.out + (size_t)i * 8, (u32x2){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3])});
+        }
+    }
+    const int e = whole * kElems + threadIdx.x;
+    if (e < p.n) store_elem<O>(p.out, e, load_elem<G>(p.g, e) * c);
+}
+template <int G>
+__device__ __forceinline__ void piece_scale_from(const GradPiece& p, float c)
+{
+    if (p.out_dtype == WQ_DTYPE_BF16) piece_scale<G, WQ_DTYPE_BF16>(p, c);
+    else if (p.out_dtype == WQ_DTYPE_F16) piece_scale<G, WQ_DTYPE_F16>(p, c);
+    else piece_scale<G, WQ_DTYPE_F32>(p, c);
+}
+
+template <typename Source>
+__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_items, const float* total,
+                                                                 const float max_norm, const float scale, const float* scale_dev)
+{
+    const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    if (slot >= n_items) return;  // uniform per workgroup
+    const float c = clip_coefficient(ldg<float>(total), max_norm, effective_scale(scale, scale_dev));
+    const GradPiece p = src.piece(xcd_chunked_item(slot, n_items, kNormPiecesPerXcdRun));
+    if (c == 1.0f && p.out == p.g) return;
+    if (p.g_dtype == WQ_DTYPE_BF16) piece_scale_from<WQ_DTYPE_BF16>(p, c);
+    else if (p.g_dtype == WQ_DTYPE_F16) piece_scale_from<WQ_DTYPE_F16>(p, c);
+    else piece_scale_from<WQ_DTYPE_F32>(p, c);
+}
+
+// ---- per-tensor descriptors -> one per piece ----------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* descs, const int64_t* __restrict__ item_start,
+                                                             const int n_desc, const int64_t n_items, const int words, int64_t* items)
+{
+    const int64_t t = ((int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x) * 256 + threadIdx.x;
+    if (t >= n_items) return;
+    const int i = find_owner(item_start, n_desc, t, n_items);
+    const int64_t* d = descs + (int64_t)i * words;
+    int64_t* o = items + t * words;
+    const int64_t at = (t - item_start[i]) * kGradItem, left = d[2] - at;
+    const int g_dtype = (int)(uint32_t)d[3], out_dtype = (int)(uint32_t)((uint64_t)d[3] >> 32);
+    o[0] = d[0] + at * dtype_bytes(g_dtype);
+    o[1] = d[1] ? d[1] + at * dtype_bytes(out_dtype) : 0;
+    o[2] = left < kGradItem ? left : kGradItem;
+    o[3] = d[3];
+    if (words == 8) {
+        o[4] = d[4] + at * 4;
+        o[5] = d[5] + at * 4;
+        o[6] = d[6] + at * 4;
+        o[7] = d[7];
+    }
+}
+
+template <typename Source>
+static void launch_partials(const Source& src, int64_t n_items, int norm, void* partials, hipStream_t st)
+{
+    if (n_items == 0) return;
+    const dim3 g = grid_for_items(n_items);
+    if (norm == WQ_NORM_2) grad_norm_partials_kernel<WQ_NORM_2><<<g, kGradThreads, 0, st>>>(src, n_items, (char*)partials);
+    else grad_norm_partials_kernel<WQ_NORM_INF><<<g, kGradThreads, 0, st>>>(src, n_items, (char*)partials);
+}
+void launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* partials, hipStream_t st)
+{
+    launch_partials(src, n_items, norm, partials, st);
+}
+
+template <typename Source>
+static void launch_norm(const Source& src, int64_t n_items, int norm, float scale, const float* scale_dev, void* workspace,
+                        float* total, hipStream_t st)
+{
+    char* partials = partials_of(workspace);
+    launch_partials(src, n_items, norm, partials, st);
+    if (norm == WQ_NORM_2) grad_norm_total_kernel<WQ_NORM_2><<<1, 1024, 0, st>>>(partials, n_items, scale, scale_dev, total);
+    else grad_norm_total_kernel<WQ_NORM_INF><<<1, 1024, 0, st>>>(partials, n_items, scale, scale_dev, total);
+}
+template <typename Source>
+static void launch_clip(const Source& src, int64_t n_items, int norm, float max_norm, float scale, const float* scale_dev,
+                        const float* given, void* workspace, float* total, hipStream_t st)
+{
+    if (!given) launch_norm(src, n_items, norm, scale, scale_dev, workspace, total, st);
+    if (n_items == 0) return;
+    grad_scale_kernel<<<grid_for_items(n_items), kGradThreads, 0, st>>>(src, n_items, given ? given : total, max_norm, scale, scale_dev);
+}
+
+static bool grad_dtype_ok(int d) { return d == WQ_DTYPE_BF16 || d == WQ_DTYPE_F16 || d == WQ_DTYPE_F32; }
+
+// per-tensor HOST descriptors -> kernel arguments; negative: an error
+static int64_t few_source(const wq_grad_desc* descs, int n_desc, bool with_out, FewSource* src)
+{
+    if (n_desc < 0 || n_desc > WQ_GRAD_FEW_MAX) return WQ_ERR_SHAPE;
+    if (n_desc && !descs) return WQ_ERR_NULL;
+    int64_t items = 0;
+    int k = 0;
+    for (int i = 0; i < n_desc; ++i) {
+        if (descs[i].n < 0) return WQ_ERR_SHAPE;
+        if (!grad_dtype_ok(descs[i].g_dtype) || (with_out && !grad_dtype_ok(descs[i].out_dtype))) return WQ_ERR_MODE;
+        if (descs[i].n == 0) continue;
+        if (!descs[i].g || (with_out && !descs[i].out)) return WQ_ERR_NULL;
+        src->d[k] = descs[i];
+        src->start[k++] = items;
+        items += cdiv64(descs[i].n, kGradItem);
+    }
+    src->start[k] = items;
+    src->n_desc = k;
+    return items;
+}
+
+}  // namespace wq
+
+using namespace wq;
+
+WQ_EXPORT int64_t wq_grad_workspace_bytes(int64_t n_items) { return n_items < 0 ? 0 : kGradControlBytes + n_items * 8; }
+
+WQ_EXPORT int wq_grad_make_items(const void* descs, const int64_t* item_start, int n_desc, int64_t n_items, int words, void* items,
+                                 void* stream)
+{
+    if (n_desc < 0 || n_items < 0 || (words != 4 && words != 8)) return WQ_ERR_SHAPE;
+    if (n_items == 0) return WQ_OK;
+    if (n_desc == 0) return WQ_ERR_SHAPE;
+    if (!descs || !item_start || !items) return WQ_ERR_NULL;
+    grad_make_items_kernel<<<grid_for_items(cdiv64(n_items, 256)), 256, 0, (hipStream_t)stream>>>(
+        (const int64_t*)descs, item_start, n_desc, n_items, words, (int64_t*)items);
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}
+
+WQ_EXPORT int wq_grad_norm_items(const void* items, int64_t n_items, int words, const int64_t* item_start, int n_desc, int norm,
+                                 float grad_scale, const float* grad_scale_dev, void* workspace, float* total, float* each,
+                                 void* stream)
+{
+    if (n_items < 0 || n_desc < 0 || (words != 4 && words != 8)) return WQ_ERR_SHAPE;
+    if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
+    if (!workspace || !total || (n_items && !items) || (each && n_desc && !item_start)) return WQ_ERR_NULL;
+    hipStream_t st = (hipStream_t)stream;
+    launch_norm(TableSource{(const int64_t*)items, words}, n_items, norm, grad_scale, grad_scale_dev, workspace, total, st);
+    if (each && n_desc) {
+        const char* partials = partials_of(workspace);
+        if (norm == WQ_NORM_2) grad_norm_each_kernel<WQ_NORM_2><<<n_desc, 64, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
+        else grad_norm_each_kernel<WQ_NORM_INF><<<n_desc, 64, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
+    }
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}
+
+WQ_EXPORT int wq_grad_norm_few(const wq_grad_desc* descs, int n_desc, int norm, float grad_scale, void* workspace, float* total,
+                               void* stream)
+{
+    if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
+    FewSource src;
+    const int64_t items = few_source(descs, n_desc, false, &src);
+    if (items < 0) return (int)items;
+    if (!workspace || !total) return WQ_ERR_NULL;
+    launch_norm(src, items, norm, grad_scale, nullptr, workspace, total, (hipStream_t)stream);
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}
+
+WQ_EXPORT int wq_grad_clip_items(const wq_grad_desc* items, int64_t n_items, int norm, float max_norm, float grad_scale,
+                                 const float* grad_scale_dev, const float* total_given, void* workspace, float* total, void* stream)
+{
+    if (n_items < 0) return WQ_ERR_SHAPE;
+    if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
+    if ((!total_given && (!workspace || !total)) || (n_items && !items)) return WQ_ERR_NULL;
+    if (n_items == 0 && total_given) return WQ_OK;
+    launch_clip(TableSource{(const int64_t*)items, 4}, n_items, norm, max_norm, grad_scale, grad_scale_dev, total_given, workspace,
+                total, (hipStream_t)stream);
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}
+
+WQ_EXPORT int wq_grad_clip_few(const wq_grad_desc* descs, int n_desc, int norm, float max_norm, float grad_scale,
+                               const float* total_given, void* workspace, float* total, void* stream)
+{
+    if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
+    FewSource src;
+    const int64_t items = few_source(descs, n_desc, true, &src);
+    if (items < 0) return (int)items;
+    if (!total_given && (!workspace || !total)) return WQ_ERR_NULL;
+    if (items == 0 && total_given) return WQ_OK;
+    launch_clip(src, items, norm, max_norm, grad_scale, nullptr, total_given, workspace, total, (hipStream_t)stream);
+    WQ_LAUNCH_CHECK();
+    return WQ_OK;
+}

@@ -1,0 +1,169 @@
+// What the gradient norm, the clip and the AdamW update share: element types, piece sources and the fold of the partial
+// norms.
+#pragma once
+
+#include "wq_common.h"
+
+namespace wq {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kGradThreads = 256;
+constexpr int kGradItem = WQ_GRAD_ITEM;
+
+// 16- and 8-byte accesses of streams whose elements have their own alignment only (a tensor inside a packed buffer starts
+// anywhere): gfx950's global accesses take any address, the type says so to the compiler.
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ u32x4 ldg16(const char* p) { return *(const WQ_GLOBAL u32x4_a2*)p; }
+__device__ __forceinline__ u32x2 ldg8(const char* p) { return *(const WQ_GLOBAL u32x2_a2*)p; }
+__device__ __forceinline__ void stg16(char* p, u32x4 v) { *(WQ_GLOBAL u32x4_a2*)p = v; }
+__device__ __forceinline__ void stg8(char* p, u32x2 v) { *(WQ_GLOBAL u32x2_a2*)p = v; }
+
+constexpr int dtype_bytes(int d) { return d == WQ_DTYPE_F32 ? 4 : 2; }
+
+template <int D>
+__device__ __forceinline__ float load_elem(const char* p, int i)
+{
+    if constexpr (D == WQ_DTYPE_F32) return ldg<float>(p + (size_t)i * 4);
+    const uint32_t h = ldg<uint16_t>(p + (size_t)i * 2);
+    if constexpr (D == WQ_DTYPE_BF16) return u2f(h << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+// two 16-bit elements of a dword
+template <int D>
+__device__ __forceinline__ f32x2 unpack2(uint32_t w)
+{
+    if constexpr (D == WQ_DTYPE_BF16) return (f32x2){bf16lo(w), bf16hi(w)};
+    return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
+}
+// One rounding, to nearest even.  The value is pinned to a register first: fused into the multiplication that made it
+// (v_fma_mixlo_f16 with a +0 addend) a product of -0 would come out as +0.
+template <int D>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    asm("" : "+v"(a));
+    asm("" : "+v"(b));
+    const f32x2 v = {a, b};
+    if constexpr (D == WQ_DTYPE_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+template <int D>
+__device__ __forceinline__ void store_elem(char* p, int i, float v)
+{
+    if constexpr (D == WQ_DTYPE_F32) stg<float>(p + (size_t)i * 4, v);
+    else stg<uint16_t>(p + (size_t)i * 2, (uint16_t)pack2<D>(v, 0.0f));
+}
+
+// ---- where a workgroup finds its piece ---------------------------------------------------------------------------
+struct GradPiece {
+    const char* g;
+    char* out;
+    int n, g_dtype, out_dtype;
+};
+// A table with one descriptor per piece; `words` is 4 (wq_grad_desc) or 8 (wq_adamw_desc, which begins alike).
+struct TableSource {
+    const int64_t* items;
+    int words;
+    __device__ __forceinline__ GradPiece piece(int64_t t) const
+    {
+        const wq_grad_desc* d = (const wq_grad_desc*)(items + t * words);
+        return {(const char*)d->g, (char*)d->out, (int)d->n, d->g_dtype, d->out_dtype};
+    }
+};
+// Per-tensor descriptors in the kernel arguments.
+struct FewSource {
+    wq_grad_desc d[WQ_GRAD_FEW_MAX];
+    int64_t start[WQ_GRAD_FEW_MAX + 1];
+    int n_desc;
+    __device__ __forceinline__ GradPiece piece(int64_t t) const
+    {
+        int lo = 0, hi = n_desc;
+        while (hi - lo > 1) {  // start[lo] <= t < start[hi]; empty tensors share their successor's start
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= t) lo = mid; else hi = mid;
+        }
+        const int64_t at = (t - start[lo]) * kGradItem;
+        const int64_t left = d[lo].n - at;
+        return {(const char*)d[lo].g + at * dtype_bytes(d[lo].g_dtype), (char*)d[lo].out + at * dtype_bytes(d[lo].out_dtype),
+                (int)(left < kGradItem ? left : kGradItem), d[lo].g_dtype, d[lo].out_dtype};
+    }
+};
+
+// ---- partial norms -------------------------------------------------------------------------------------------------
+// 2-norm: a partial is a sum of squares (double).  Infinity norm: the largest magnitude's fp32 bits (integers order like
+// magnitudes and NaN is above infinity, so a NaN wins), as a uint64.
+template <int NORM> struct NormAcc;
+template <> struct NormAcc<WQ_NORM_2> {
+    typedef double T;
+    static __device__ __forceinline__ T zero() { return 0.0; }
+    static __device__ __forceinline__ T join(T a, T b) { return a + b; }
+    static __device__ __forceinline__ void add(T& a, float x)
+    {
+        const double d = (double)x;
+        a = __builtin_fma(d, d, a);
+    }
+    static __device__ __forceinline__ float finish(T a, float scale) { return (float)(__builtin_sqrt(a) * (double)__builtin_fabsf(scale)); }
+};
+template <> struct NormAcc<WQ_NORM_INF> {
+    typedef uint64_t T;
+    static __device__ __forceinline__ T zero() { return 0; }
+    static __device__ __forceinline__ T join(T a, T b) { return a > b ? a : b; }
+    static __device__ __forceinline__ void add(T& a, float x) { a = (uint64_t)max((uint32_t)a, f2u(x) & 0x7FFFFFFFu); }
+    static __device__ __forceinline__ float finish(T a, float scale) { return u2f((uint32_t)a) * __builtin_fabsf(scale); }
+};
+
+template <typename T>
+__device__ __forceinline__ T shfl_xor_64(T v, int m)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, m), hi = (uint32_t)__shfl_xor((int)(uint32_t)(b >> 32), m);
+    return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
+}
+template <int NORM>
+__device__ __forceinline__ typename NormAcc<NORM>::T wave_fold(typename NormAcc<NORM>::T a)
+{
+#pragma unroll
+    for (int m = 32; m; m >>= 1) a = NormAcc<NORM>::join(a, shfl_xor_64(a, m));
+    return a;
+}
+// The fold over a workgroup of WAVES wavefronts; valid in every lane.  lds: WAVES values.
+template <int NORM, int WAVES>
+__device__ __forceinline__ typename NormAcc<NORM>::T block_fold(typename NormAcc<NORM>::T a, typename NormAcc<NORM>::T* lds)
+{
+    a = wave_fold<NORM>(a);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = lds[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) a = NormAcc<NORM>::join(a, lds[w]);
+    return a;
+}
+
+// The fold of all partials by one workgroup of 1024, in an order that depends on their number only.
+template <int NORM>
+__device__ __forceinline__ typename NormAcc<NORM>::T fold_partials(const void* partials, int64_t n, typename NormAcc<NORM>::T* lds)
+{
+    typedef typename NormAcc<NORM>::T T;
+    T a = NormAcc<NORM>::zero();
+    for (int64_t i = threadIdx.x; i < n; i += 1024) a = NormAcc<NORM>::join(a, ldg<T>((const char*)partials + i * 8));
+    return block_fold<NORM, 16>(a, lds);
+}
+
+__device__ __forceinline__ float effective_scale(float scale, const float* dev) { return dev ? scale * ldg<float>(dev) : scale; }
+__device__ __forceinline__ float clip_coefficient(float norm, float max_norm, float scale)
+{
+    const float c = max_norm / (norm + 1e-6f);
+    return (c > 1.0f ? 1.0f : c) * scale;      // NaN stays NaN
+}
+
+// workspace: 64 bytes of AdamW's per-step values, then the partials
+constexpr int64_t kGradControlBytes = 64;
+inline char* partials_of(void* workspace) { return (char*)workspace + kGradControlBytes; }
+
+// wq_grad.hip: one partial per piece
+void launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* partials, hipStream_t st);
+
+}  // namespace wq

@@ -1,0 +1,467 @@
+"""What lies between a backward pass and the quantisers: the global gradient norm, clipping by it and the AdamW update.
+
+The trainer's loop around a weight sync is backward -> norm -> clip -> update -> quantise -> ship, and everything here works
+like the quantisers do: over whole lists of tensors, a few launches per list, nothing read back to the host.  The update takes
+the clip as a factor (no pass of its own) and writes the bf16 / fp16 weight that ``Fp8QuantPlan``, ``Int4PackPlan`` or
+``BucketConverter`` then read.
+
+``get_total_norm``, ``clip_grad_norm_`` and ``clip_grads_with_norm_`` have the names and arguments of ``torch.nn.utils`` and take
+whatever gradients a call presents; ``GradNormPlan``, ``GradClipPlan`` and ``AdamWPlan`` take a fixed list (gradient buffers that
+stay where they are) and can be captured into a HIP graph.  Norms are fp32, whatever the gradients' type: sums of squares are
+formed in 64 bits in a fixed order, so they neither overflow nor depend on the run.
+
+Norm of a model that is sharded over ranks: ``norm = plan.run(); total = norm.square(); all_reduce(total);`` and
+``total_norm=total.sqrt()`` in the clip or the update.
+"""
+
+from __future__ import annotations
+
+import array
+import math
+from typing import Iterable, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_NORMS = {2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
+
+
+def _norm_selector(norm_type, what: str) -> int:
+    norm = _NORMS.get(float(norm_type))
+    if norm is None:
+        raise ValueError(f"{what}: norm_type {norm_type} is not supported (2 and inf are)")
+    return norm
+
+
+def _check_max_norm(max_norm, what: str) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm must not be negative or NaN, got {max_norm}")
+    return max_norm
+
+
+def _check_tensor(t, what: str, dtypes=_DTYPES) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.layout != torch.strided or hasattr(t, "to_local"):
+        raise TypeError(f"{what}: only plain strided tensors are supported (of a sharded one, pass the local part)")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what}: dtype {t.dtype} is not supported ({', '.join(str(d) for d in dtypes)})")
+
+
+def _strides(t):
+    """(stride, size) of the dimensions that have a stride, smallest first."""
+    return sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1)
+
+
+def _is_dense(t) -> bool:
+    """Whether the elements fill one run of memory, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for st, n in _strides(t):
+        if st != expected:
+            return False
+        expected *= n
+    return True
+
+
+def _check_no_self_overlap(t, what: str) -> None:
+    reach = 0
+    for st, n in _strides(t):
+        if st <= reach:
+            raise ValueError(f"{what}: elements of a gradient share memory (strides {tuple(t.stride())}); it cannot be written")
+        reach += st * (n - 1)
+
+
+def _same_layout(a, b) -> bool:
+    return a.shape == b.shape and (a.stride() == b.stride() or a.numel() == 0 or
+                                   all(n == 1 or x == y for x, y, n in zip(a.stride(), b.stride(), a.shape)))
+
+
+def _one_device(tensors, what: str) -> torch.device:
+    device = tensors[0].device
+    for t in tensors:
+        _lib.require_gpu(t, what)
+        if t.device != device:
+            raise ValueError(f"{what}: all tensors must be on one device (got {device} and {t.device})")
+    return device
+
+
+def _refuse_overlaps(written, read, what: str) -> None:
+    """Ranges that are written share no byte with each other or with one that is read."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w)
+             for ts, w in ((written, True), (read, False)) for t in ts if t.numel()]
+    if not spans:
+        return
+    a = np.array(spans, dtype=np.int64)
+    a = a[np.lexsort((a[:, 1], a[:, 0]))]
+    end, w = a[:, 1], a[:, 2].astype(bool)
+    any_end = np.maximum.accumulate(end)[:-1]
+    written_end = np.maximum.accumulate(np.where(w, end, 0))[:-1]
+    if ((a[1:, 0] < written_end) | (w[1:] & (a[1:, 0] < any_end))).any():
+        raise ValueError(f"{what}: tensors that are written share memory with others of the call (the same tensor twice?)")
+
+
+def _scalar_on_device(value, device, what: str):
+    if value.dtype != torch.float32 or value.numel() != 1 or value.device != device:
+        raise ValueError(f"{what} must be a number or one float32 value on {device}")
+    return value.data_ptr()
+
+
+def _scale_args(scale, device, what: str):
+    """-> (factor, address of a factor on the device or None)"""
+    if isinstance(scale, torch.Tensor):
+        return 1.0, _scalar_on_device(scale, device, what)
+    scale = float(scale)
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"{what} must be a finite number that is not negative, got {scale}")
+    return scale, None
+
+
+def _launch(device: torch.device, entry: str, what: str, *args) -> None:
+    fn = getattr(_lib.load(), entry)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _lib.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_ptr(device))
+    _lib.check(rc, what)
+
+
+def _bump(tensors) -> None:
+    """Tell autograd that a kernel wrote into these tensors, as torch's in-place operations do."""
+    tensors = [t for t in tensors if not t.is_inference()]
+    if tensors:
+        torch.autograd.graph.increment_version(tensors)
+
+
+def _pieces(n: int) -> int:
+    return -(-n // _lib.GRAD_ITEM)
+
+
+def _workspace(n_items: int, device) -> torch.Tensor:
+    return torch.empty(_lib.load().wq_grad_workspace_bytes(n_items) // 8, dtype=torch.int64, device=device)
+
+
+def _grad_row(g, out=None):
+    out = g if out is None else out
+    return [g.data_ptr(), out.data_ptr(), g.numel(), _DTYPES[g.dtype] | _DTYPES[out.dtype] << 32]
+
+
+def _item_table(rows: np.ndarray, device, what: str, wait: bool):
+    """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
+    of the tensors in it).  Without ``wait`` the upload goes through pinned memory and the host goes on."""
+    starts = np.zeros(len(rows) + 1, dtype=np.int64)
+    np.cumsum(-(-rows[:, 2] // _lib.GRAD_ITEM), out=starts[1:])
+    host = torch.from_numpy(np.concatenate([rows.reshape(-1), starts]))
+    if wait:
+        table = host.to(device)
+    else:
+        table = host.pin_memory().to(device, non_blocking=True)
+    n_items, words = int(starts[-1]), rows.shape[1]
+    items = torch.empty((max(n_items, 1), words), dtype=torch.int64, device=device)
+    start_t = table[rows.size:]
+    _launch(device, "wq_grad_make_items", what, table.data_ptr(), start_t.data_ptr(), len(rows), n_items, words, items.data_ptr())
+    return items, start_t, n_items
+
+
+class _Plan:
+    """Tables and workspace of a fixed list.  One plan's runs must be ordered on one stream (or by events): they share the
+    workspace.  A run on another stream than the one the plan was built on is fine."""
+
+    def _build(self, rows, device, what: str) -> None:
+        self.device, self._what = device, what
+        with torch.cuda.device(device):
+            self._items, self._starts, self._n_items = _item_table(np.array(rows, dtype=np.int64), device, what, wait=True)
+            self._workspace = _workspace(self._n_items, device)
+            self.total_norm = torch.zeros((), dtype=torch.float32, device=device)
+            self._stream = torch.cuda.current_stream(device)
+            self._owned = [self._items, self._starts, self._workspace, self.total_norm]
+
+    def _built(self) -> None:
+        self._stream.synchronize()      # a run on another stream finds the tables ready
+
+    def _run(self, entry: str, *args) -> None:
+        stream = torch.cuda.current_stream(self.device)
+        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+            for t in self._owned:       # the allocator must not hand them out while this stream may still use them
+                t.record_stream(stream)
+        _launch(self.device, entry, self._what, *args)
+
+    def _given(self, total_norm):
+        return None if total_norm is None else _scalar_on_device(total_norm, self.device, f"{self._what}: total_norm")
+
+
+def _check_grads(grads, what: str):
+    grads = list(grads)
+    if not grads:
+        raise ValueError(f"{what}: empty gradient list")
+    for g in grads:
+        _check_tensor(g, what)
+        if not _is_dense(g):
+            raise ValueError(f"{what}: tensors of a plan must fill one run of memory (a copy would be read instead of the live "
+                             f"gradient); got shape {tuple(g.shape)}, strides {tuple(g.stride())}")
+    return grads
+
+
+class GradNormPlan(_Plan):
+    """The global norm (2 or inf) of a fixed list of bf16 / fp16 / fp32 gradients, and with ``per_tensor`` the norm of each.
+
+    ``run(grad_scale=1.0)`` returns ``total_norm``, a 0-d fp32 tensor that the next run overwrites, or ``(total_norm, norms)``
+    with ``norms`` fp32 ``[len(grads)]``.  grad_scale (a number or one fp32 value on the device: an inverse loss scale, one over
+    the number of tokens) multiplies the gradients.  A gradient may be in the list twice and then counts twice."""
+
+    def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_tensor: bool = False):
+        self._norm = _norm_selector(norm_type, "GradNormPlan")
+        self.grads = _check_grads(grads, "GradNormPlan")
+        self._build([_grad_row(g) for g in self.grads], _one_device(self.grads, "GradNormPlan"), "GradNormPlan")
+        self.norms = torch.zeros(len(self.grads), dtype=torch.float32, device=self.device) if per_tensor else None
+        if per_tensor:
+            self._owned.append(self.norms)
+        self._built()
+
+    def run(self, grad_scale=1.0):
+        scale, scale_dev = _scale_args(grad_scale, self.device, "GradNormPlan: grad_scale")
+        each = self.norms
+        self._run("wq_grad_norm_items", self._items.data_ptr(), self._n_items, 4, self._starts.data_ptr(), len(self.grads),
+                  self._norm, scale, scale_dev, self._workspace.data_ptr(), self.total_norm.data_ptr(),
+                  None if each is None else each.data_ptr())
+        return self.total_norm if each is None else (self.total_norm, each)
+
+
+class GradClipPlan(_Plan):
+    """Clip a fixed list of gradients by their global norm: ``g * grad_scale * min(1, max_norm / (norm + 1e-6))``, in place or,
+    with ``out``, into other tensors of the same shapes and layouts (bf16 gradients into fp32 main gradients, say), rounded
+    once.  In place, gradients that need no change are not rewritten.
+
+    ``run(max_norm, grad_scale=1.0, total_norm=None)`` returns the norm before the clip (of the scaled gradients): a 0-d fp32
+    tensor that the next run overwrites, or the ``total_norm`` it was given."""
+
+    def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, out: Sequence[torch.Tensor] | None = None):
+        self._norm = _norm_selector(norm_type, "GradClipPlan")
+        self.grads = _check_grads(grads, "GradClipPlan")
+        self.out = self.grads if out is None else list(out)
+        if len(self.out) != len(self.grads):
+            raise ValueError("GradClipPlan: need one output per gradient")
+        for g, o in zip(self.grads, self.out):
+            _check_tensor(o, "GradClipPlan")
+            if not _same_layout(g, o):
+                raise ValueError(f"GradClipPlan: output of shape {tuple(o.shape)}, strides {tuple(o.stride())} for a gradient of "
+                                 f"shape {tuple(g.shape)}, strides {tuple(g.stride())}")
+        apart = [g for g, o in zip(self.grads, self.out) if g.data_ptr() != o.data_ptr() or g.dtype != o.dtype]
+        _refuse_overlaps(self.out, apart, "GradClipPlan")
+        device = _one_device(self.grads + self.out, "GradClipPlan")
+        self._build([_grad_row(g, o) for g, o in zip(self.grads, self.out)], device, "GradClipPlan")
+        self._built()
+
+    def run(self, max_norm: float, grad_scale=1.0, total_norm: torch.Tensor | None = None) -> torch.Tensor:
+        max_norm = _check_max_norm(max_norm, "GradClipPlan")
+        scale, scale_dev = _scale_args(grad_scale, self.device, "GradClipPlan: grad_scale")
+        self._run("wq_grad_clip_items", self._items.data_ptr(), self._n_items, self._norm, max_norm, scale, scale_dev,
+                  self._given(total_norm), self._workspace.data_ptr(), self.total_norm.data_ptr())
+        _bump(self.out)
+        return self.total_norm if total_norm is None else total_norm
+
+
+def _per_tensor(value, n: int, what: str):
+    values = [float(value)] * n if isinstance(value, (int, float)) else [float(v) for v in value]
+    if len(values) != n:
+        raise ValueError(f"AdamWPlan: need one {what} per parameter")
+    for v in values:
+        if not 0.0 <= v < math.inf:
+            raise ValueError(f"AdamWPlan: {what} must be finite and not negative, got {v}")
+    return values
+
+
+class AdamWPlan(_Plan):
+    """One AdamW step (decoupled weight decay) over a fixed list of fp32 parameters per ``run()``: with t = ``step`` + 1 and
+    g = gradient * grad_scale * min(1, max_norm / (norm + 1e-6)),
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        p = p - lr w p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps);  weight = round(p)
+
+    ``weights``: bf16 / fp16 copies of the parameters (None, or None for single ones), written by the same pass.
+    ``exp_avgs`` / ``exp_avg_sqs``: fp32 moments (fresh zeros by default).  All tensors of one parameter have its shape and
+    layout.  ``weight_decay`` (w) and ``lr_scale`` (multiplies lr): one number or one per parameter.  ``step`` counts the steps
+    done, in a 0-d int64 tensor on the device (``plan.step``; start at another one with ``step=``), so a captured run counts its
+    replays.  With ``skip_nonfinite`` a step whose gradient norm is infinite or NaN changes nothing and is not counted.
+
+    ``run(lr, max_norm=None, grad_scale=1.0, total_norm=None)``: lr is a number or one fp32 value on the device (a number is
+    fixed in a captured run).  Returns the gradient norm before the clip where it is needed (max_norm or skip_nonfinite; a 0-d
+    fp32 tensor that the next run overwrites, or the ``total_norm`` given), else None."""
+
+    def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], weights: Sequence | None = None,
+                 exp_avgs: Sequence[torch.Tensor] | None = None, exp_avg_sqs: Sequence[torch.Tensor] | None = None,
+                 betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0, norm_type: float = 2.0,
+                 skip_nonfinite: bool = False, step: int = 0):
+        self._norm = _norm_selector(norm_type, "AdamWPlan")
+        self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
+        if not all(0.0 <= b < 1.0 for b in self.betas) or not 0.0 <= self.eps < math.inf:
+            raise ValueError(f"AdamWPlan: betas must be in [0, 1) and eps finite and not negative, got {betas}, {eps}")
+        if int(step) < 0:
+            raise ValueError(f"AdamWPlan: step must not be negative, got {step}")
+        self.grads, self.params = _check_grads(grads, "AdamWPlan"), list(params)
+        n = len(self.params)
+        self.weights = [None] * n if weights is None else list(weights)
+        given = [self.params, self.grads, self.weights] + [list(x) for x in (exp_avgs, exp_avg_sqs) if x is not None]
+        if any(len(x) != n for x in given):
+            raise ValueError("AdamWPlan: need equally many parameters, gradients, weights and moments")
+        decay, lr_scales = _per_tensor(weight_decay, n, "weight_decay"), _per_tensor(lr_scale, n, "lr_scale")
+        for p in self.params:
+            _check_tensor(p, "AdamWPlan: parameters", (torch.float32,))
+        moments = [[None] * n if x is None else list(x) for x in (exp_avgs, exp_avg_sqs)]
+        for p, g, w, m, v in zip(self.params, self.grads, self.weights, *moments):
+            for x in (m, v):
+                if x is not None:
+                    _check_tensor(x, "AdamWPlan: moments", (torch.float32,))
+            if w is not None:
+                _check_tensor(w, "AdamWPlan: weights", (torch.bfloat16, torch.float16))
+            if not all(_same_layout(p, x) for x in (g, w, m, v) if x is not None):
+                raise ValueError(f"AdamWPlan: gradient, weight and moments must have the shape and strides of their parameter "
+                                 f"({tuple(p.shape)}, {tuple(p.stride())})")
+        self._written = self.params + [w for w in self.weights if w is not None]
+        state = [x for xs in moments for x in xs if x is not None]
+        _refuse_overlaps(self._written + state, self.grads, "AdamWPlan")
+        device = _one_device(self.params + self.grads + self._written + state, "AdamWPlan")
+        # fresh moments in the parameter's layout
+        moments = [[torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=device).zero_() if x is None else x
+                    for p, x in zip(self.params, xs)] for xs in moments]
+        self.exp_avgs, self.exp_avg_sqs = moments
+        floats = np.array([lr_scales, decay], dtype=np.float32).T.copy().view(np.int64).reshape(-1)
+        rows = [[g.data_ptr(), 0 if w is None else w.data_ptr(), p.numel(), _DTYPES[g.dtype] | (0 if w is None else _DTYPES[w.dtype]) << 32,
+                 p.data_ptr(), m.data_ptr(), v.data_ptr(), int(f)]
+                for p, g, w, m, v, f in zip(self.params, self.grads, self.weights, self.exp_avgs, self.exp_avg_sqs, floats)]
+        self._build(rows, device, "AdamWPlan")
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self.step = torch.full((), int(step), dtype=torch.int64, device=device)
+        self._owned.append(self.step)
+        self._built()
+
+    def run(self, lr, max_norm: float | None = None, grad_scale=1.0, total_norm: torch.Tensor | None = None):
+        max_norm = -1.0 if max_norm is None else _check_max_norm(max_norm, "AdamWPlan")
+        scale, scale_dev = _scale_args(grad_scale, self.device, "AdamWPlan: grad_scale")
+        lr, lr_dev = _scale_args(lr, self.device, "AdamWPlan: lr")
+        hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, lr, lr_dev, scale_dev, self._given(total_norm),
+                                self.total_norm.data_ptr(), self.step.data_ptr(), scale, max_norm, self._norm, self.skip_nonfinite)
+        self._run("wq_adamw_items", self._items.data_ptr(), self._n_items, hyper, self._workspace.data_ptr())
+        _bump(self._written)
+        if max_norm < 0.0 and not self.skip_nonfinite:
+            return None
+        return self.total_norm if total_norm is None else total_norm
+
+
+# ---- the torch.nn.utils forms ---------------------------------------------------------------------------------------
+
+def _grads_of(parameters) -> list:
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return [p.grad for p in parameters if p.grad is not None]
+
+
+def _checked(tensors, what: str):
+    for t in tensors:
+        _check_tensor(t, what)
+    return _one_device(tensors, what)
+
+
+def _call(tensors, device, few: str, many: str, what: str, few_args, many_args) -> None:
+    """The launch over ``tensors``: descriptors in the kernel arguments, or a table made for this call."""
+    n = len(tensors)
+    rows = [_grad_row(t) for t in tensors]
+    if n <= _lib.GRAD_FEW_MAX:
+        host = array.array("q", [x for row in rows for x in row])
+        _launch(device, few, what, host.buffer_info()[0], n, *few_args)
+        return
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: a call over more than {_lib.GRAD_FEW_MAX} tensors cannot be captured; use a plan")
+    with torch.cuda.device(device):
+        items, starts, n_items = _item_table(np.array(rows, dtype=np.int64), device, what, wait=False)
+    _launch(device, many, what, *many_args(items.data_ptr(), starts.data_ptr(), n_items, n))
+
+
+def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
+    if not torch.isfinite(total):
+        raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients is non-finite, so it cannot be clipped. "
+                           "To disable this error and scale the gradients by the non-finite norm anyway, set "
+                           "`error_if_nonfinite=False`")
+
+
+def _total_norm(tensors, device, norm: int, what: str) -> torch.Tensor:
+    dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
+    total = torch.empty((), dtype=torch.float32, device=device)
+    ws = _workspace(sum(_pieces(t.numel()) for t in dense), device)
+    _call(dense, device, "wq_grad_norm_few", "wq_grad_norm_items", what, (norm, 1.0, ws.data_ptr(), total.data_ptr()),
+          lambda items, starts, n_items, n: (items, n_items, 4, starts, n, norm, 1.0, None, ws.data_ptr(), total.data_ptr(), None))
+    return total
+
+
+def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                   foreach: bool | None = None) -> torch.Tensor:
+    """``torch.nn.utils.get_total_norm`` for bf16 / fp16 / fp32 tensors on one GPU: the norm (2 or inf) over all elements as a
+    0-d fp32 tensor (torch rounds it to the tensors' type).  ``foreach`` is accepted and has no effect."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    norm = _norm_selector(norm_type, "get_total_norm")
+    if not tensors:
+        return torch.tensor(0.0)
+    total = _total_norm(tensors, _checked(tensors, "get_total_norm"), norm, "get_total_norm")
+    if error_if_nonfinite:
+        _refuse_nonfinite(total, norm_type)
+    return total
+
+
+def _clip(grads, max_norm: float, norm: int, total_norm, what: str) -> torch.Tensor:
+    device = _checked(grads, what)
+    dense, copies = [], []
+    for g in grads:
+        if _is_dense(g):
+            dense.append(g)
+        else:
+            _check_no_self_overlap(g, what)
+            copies.append((g, g.contiguous()))
+    _refuse_overlaps(dense, (), what)
+    work = dense + [c for _, c in copies]
+    if total_norm is None:
+        total = torch.empty((), dtype=torch.float32, device=device)
+        ws, given = _workspace(sum(_pieces(g.numel()) for g in work), device).data_ptr(), None
+    else:
+        total = total_norm.detach().to(device=device, dtype=torch.float32)
+        ws, given = None, total.data_ptr()
+    _call(work, device, "wq_grad_clip_few", "wq_grad_clip_items", what, (norm, max_norm, 1.0, given, ws, total.data_ptr()),
+          lambda items, _, n_items, n: (items, n_items, norm, max_norm, 1.0, None, given, ws, total.data_ptr()))
+    _bump(dense)
+    for g, c in copies:
+        g.copy_(c)
+    return total
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` for bf16 / fp16 / fp32 gradients on one GPU: scales the gradients in place by
+    ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before the clip as a 0-d fp32 tensor.  Nothing is read back
+    unless ``error_if_nonfinite``.  The gradients must not share memory.  ``foreach`` is accepted and has no effect."""
+    norm, max_norm = _norm_selector(norm_type, "clip_grad_norm_"), _check_max_norm(max_norm, "clip_grad_norm_")
+    grads = _grads_of(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    total = None
+    if error_if_nonfinite:
+        total = _total_norm(grads, _checked(grads, "clip_grad_norm_"), norm, "clip_grad_norm_")
+        _refuse_nonfinite(total, norm_type)
+    return _clip(grads, max_norm, norm, total, "clip_grad_norm_")
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor,
+                          foreach: bool | None = None) -> None:
+    """``torch.nn.utils.clip_grads_with_norm_``: the clip alone, by a norm that the caller has (reduced over ranks, say)."""
+    max_norm = _check_max_norm(max_norm, "clip_grads_with_norm_")
+    if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1:
+        raise TypeError("clip_grads_with_norm_: total_norm must be a tensor of one value")
+    grads = _grads_of(parameters)
+    if grads:
+        _clip(grads, max_norm, _lib.NORM_2, total_norm, "clip_grads_with_norm_")

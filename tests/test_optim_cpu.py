@@ -1,0 +1,258 @@
+"""Refusals and host logic of the gradient norm, the clip and the AdamW update (no GPU needed: everything here is decided
+before a launch)."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import slime_amd
+from slime_amd import _lib, optim
+
+S, M_, N_ = -2, -3, -1
+P = ctypes.c_void_p(64)      # a pointer that is never followed
+
+
+def _lists(n=3, dtype=torch.float32, shape=(4, 8)):
+    return [torch.zeros(shape, dtype=dtype) for _ in range(n)]
+
+
+# ---- C ABI ---------------------------------------------------------------------------------------------------------------
+def test_entry_points_reject_bad_arguments():
+    lib = _lib.load()
+    assert lib.wq_grad_workspace_bytes(-1) == 0 and lib.wq_grad_workspace_bytes(0) >= 64
+    assert lib.wq_grad_workspace_bytes(1000) >= 8000
+    assert lib.wq_grad_make_items(None, None, 1, -1, 4, None, None) == S
+    assert lib.wq_grad_make_items(None, None, 1, 3, 5, None, None) == S
+    assert lib.wq_grad_make_items(None, None, 0, 3, 4, None, None) == S
+    assert lib.wq_grad_make_items(None, None, 1, 3, 4, None, None) == N_
+    assert lib.wq_grad_make_items(None, None, 0, 0, 4, None, None) == 0
+    assert lib.wq_grad_norm_items(None, -1, 4, None, 0, 0, 1.0, None, P, P, None, None) == S
+    assert lib.wq_grad_norm_items(None, 1, 6, None, 0, 0, 1.0, None, P, P, None, None) == S
+    assert lib.wq_grad_norm_items(P, 1, 4, None, 0, 2, 1.0, None, P, P, None, None) == M_
+    assert lib.wq_grad_norm_items(None, 1, 4, None, 0, 0, 1.0, None, P, P, None, None) == N_
+    assert lib.wq_grad_norm_items(P, 1, 4, None, 0, 0, 1.0, None, None, P, None, None) == N_
+    assert lib.wq_grad_norm_items(P, 1, 4, None, 0, 0, 1.0, None, P, None, None, None) == N_
+    assert lib.wq_grad_norm_items(P, 1, 4, None, 2, 0, 1.0, None, P, P, P, None) == N_          # `each` without the starts
+    assert lib.wq_grad_norm_few(None, _lib.GRAD_FEW_MAX + 1, 0, 1.0, P, P, None) == S
+    assert lib.wq_grad_norm_few(None, -1, 0, 1.0, P, P, None) == S
+    assert lib.wq_grad_norm_few(None, 2, 0, 1.0, P, P, None) == N_
+    assert lib.wq_grad_norm_few(None, 0, 7, 1.0, P, P, None) == M_
+    assert lib.wq_grad_norm_few(None, 0, 0, 1.0, None, P, None) == N_
+    assert lib.wq_grad_clip_items(None, 2, 0, 1.0, 1.0, None, None, P, P, None) == N_
+    assert lib.wq_grad_clip_items(P, 2, 0, 1.0, 1.0, None, None, None, P, None) == N_
+    assert lib.wq_grad_clip_items(P, -2, 0, 1.0, 1.0, None, P, None, None, None) == S
+    assert lib.wq_grad_clip_items(P, 2, 5, 1.0, 1.0, None, P, None, None, None) == M_
+    assert lib.wq_grad_clip_items(None, 0, 0, 1.0, 1.0, None, P, None, None, None) == 0         # nothing to do
+    assert lib.wq_grad_clip_few(None, 3, 0, 1.0, 1.0, P, None, None, None) == N_
+    assert lib.wq_grad_clip_few(None, 0, 0, 1.0, 1.0, P, None, None, None) == 0
+
+
+def _few(**change):
+    d = {"g": 64, "out": 64, "n": 5, "g_dtype": _lib.DTYPE_F32, "out_dtype": _lib.DTYPE_F32}
+    d.update(change)
+    return (ctypes.c_int64 * 4)(d["g"], d["out"], d["n"], d["g_dtype"] | d["out_dtype"] << 32)
+
+
+def test_host_descriptors_are_checked():
+    lib = _lib.load()
+    norm = lambda d: lib.wq_grad_norm_few(d, 1, 0, 1.0, None, None, None)      # noqa: E731  stops at the missing workspace
+    clip = lambda d: lib.wq_grad_clip_few(d, 1, 0, 1.0, 1.0, None, None, None, None)  # noqa: E731
+    assert norm(_few()) == clip(_few()) == N_
+    assert norm(_few(n=-1)) == clip(_few(n=-1)) == S
+    assert norm(_few(g_dtype=_lib.DTYPE_F64)) == clip(_few(g_dtype=9)) == M_
+    assert clip(_few(out_dtype=_lib.DTYPE_F64)) == M_
+    assert norm(_few(out_dtype=_lib.DTYPE_F64, out=0)) == N_                    # a norm looks at neither
+    assert clip(_few(out=0)) == N_ and norm(_few(g=0)) == N_
+
+
+def _hyper(**change):
+    h = dict(beta1=0.9, beta2=0.999, eps=1e-8, lr=1e-3, lr_dev=None, grad_scale_dev=None, total_given=None, total=None, step=64,
+             grad_scale=1.0, max_norm=-1.0, norm=0, skip_nonfinite=0)
+    h.update(change)
+    return _lib.AdamWHyper(**h)
+
+
+def test_adamw_entry_point_rejects_bad_arguments():
+    call = lambda h, items=P, n=1, ws=P: _lib.load().wq_adamw_items(items, n, h, ws, None)      # noqa: E731
+    assert call(_hyper(), n=-1) == S
+    assert call(None) == N_ and call(_hyper(), items=None) == N_ and call(_hyper(), ws=None) == N_ and call(_hyper(step=None)) == N_
+    assert call(_hyper(norm=3)) == M_
+    for bad in ({"beta1": 1.0}, {"beta1": -0.1}, {"beta2": 1.5}, {"beta2": math.nan}, {"eps": -1.0}, {"eps": math.nan}):
+        assert call(_hyper(**bad)) == S, bad
+    assert call(_hyper(max_norm=1.0)) == N_ and call(_hyper(skip_nonfinite=1)) == N_            # a norm, and nowhere to put it
+
+
+def test_structs_match_the_header():
+    assert ctypes.sizeof(_lib.AdamWHyper) == 4 * 8 + 5 * 8 + 4 * 4
+
+
+# ---- Python refusals ------------------------------------------------------------------------------------------------------
+PLANS = [lambda g, **k: optim.GradNormPlan(g, **k), lambda g, **k: optim.GradClipPlan(g, **k),
+         lambda g, **k: optim.AdamWPlan([torch.zeros(getattr(x, "shape", 1)) for x in g], g, **k)]
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_plans_refuse(plan):
+    with pytest.raises(RuntimeError, match="GPU"):
+        plan(_lists())
+    with pytest.raises(ValueError, match="empty"):
+        plan([])
+    with pytest.raises(ValueError, match="norm_type"):
+        plan(_lists(), norm_type=1.0)
+    with pytest.raises(TypeError, match="dtype"):
+        plan(_lists(dtype=torch.float64))
+    with pytest.raises(TypeError, match="dtype"):
+        plan(_lists(dtype=torch.int32))
+    with pytest.raises(TypeError, match="expected a tensor"):
+        plan([None])
+    with pytest.raises(TypeError, match="strided"):
+        plan([torch.zeros(4, 4).to_sparse()])
+    with pytest.raises(ValueError, match="one run"):
+        plan([torch.zeros(4, 8)[:, :5]])
+    with pytest.raises(ValueError, match="one run"):
+        plan([torch.zeros(4, 1).expand(4, 8)])
+
+
+@pytest.mark.parametrize("call", [lambda g: slime_amd.get_total_norm(g), lambda g: slime_amd.get_total_norm(g[0]),
+                                  lambda g: slime_amd.clip_grad_norm_(_params(g), 1.0),
+                                  lambda g: slime_amd.clip_grad_norm_(_params(g)[0], 1.0, error_if_nonfinite=True),
+                                  lambda g: slime_amd.clip_grads_with_norm_(_params(g), 1.0, torch.ones(()))])
+def test_functions_refuse_host_tensors_and_types(call):
+    with pytest.raises(RuntimeError, match="GPU"):
+        call(_lists())
+    with pytest.raises(TypeError, match="dtype"):
+        call(_lists(dtype=torch.float64))
+
+
+def _params(grads):
+    ps = [torch.nn.Parameter(torch.zeros(g.shape, dtype=g.dtype)) for g in grads]
+    for p, g in zip(ps, grads):
+        p.grad = g
+    return ps
+
+
+def test_functions_check_their_numbers():
+    ps = _params(_lists())
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            slime_amd.clip_grad_norm_(ps, bad)
+        with pytest.raises(ValueError, match="max_norm"):
+            slime_amd.clip_grads_with_norm_(ps, bad, torch.ones(()))
+    with pytest.raises(ValueError, match="norm_type"):
+        slime_amd.clip_grad_norm_(ps, 1.0, norm_type=3)
+    with pytest.raises(ValueError, match="norm_type"):
+        slime_amd.get_total_norm(_lists(), 1)
+    with pytest.raises(TypeError, match="total_norm"):
+        slime_amd.clip_grads_with_norm_(ps, 1.0, 2.0)
+
+
+def test_nothing_to_do_needs_no_gpu():
+    assert slime_amd.get_total_norm([]).item() == 0.0
+    assert slime_amd.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0).item() == 0.0
+    assert slime_amd.clip_grad_norm_(iter([]), 1.0).item() == 0.0
+    assert slime_amd.clip_grads_with_norm_([], 1.0, torch.ones(())) is None
+
+
+def test_clip_plan_checks_its_outputs():
+    g = _lists()
+    with pytest.raises(ValueError, match="one output"):
+        optim.GradClipPlan(g, out=_lists(2))
+    with pytest.raises(ValueError, match="output of shape"):
+        optim.GradClipPlan(g, out=_lists(shape=(8, 4)))
+    with pytest.raises(ValueError, match="output of shape"):
+        optim.GradClipPlan(g, out=[x.t().contiguous().t() for x in _lists()])
+    with pytest.raises(TypeError, match="dtype"):
+        optim.GradClipPlan(g, out=_lists(dtype=torch.float64))
+    with pytest.raises(ValueError, match="share memory"):
+        optim.GradClipPlan([g[0], g[1], g[0]])
+    with pytest.raises(ValueError, match="share memory"):
+        optim.GradClipPlan(g, out=[g[1], g[0], g[2]])                    # each other's
+    buf = torch.zeros(40)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.GradClipPlan([buf[0:8], buf[16:24]], out=[buf[32:40], buf[30:38]])
+    with pytest.raises(RuntimeError, match="GPU"):                        # neighbours, and in place next to apart: fine so far
+        optim.GradClipPlan([buf[0:8], buf[8:16]], out=[buf[0:8], buf[16:24]])
+
+
+def test_adamw_plan_checks_its_lists():
+    p, g = _lists(), _lists()
+    make = lambda **k: optim.AdamWPlan(p, g, **k)      # noqa: E731
+    with pytest.raises(ValueError, match="equally many"):
+        optim.AdamWPlan(p, _lists(2))
+    with pytest.raises(ValueError, match="equally many"):
+        make(weights=_lists(2, torch.bfloat16))
+    with pytest.raises(ValueError, match="equally many"):
+        make(exp_avgs=_lists(4))
+    for bad in ({"betas": (1.0, 0.9)}, {"betas": (0.9, -0.1)}, {"betas": (math.nan, 0.9)}, {"eps": -1.0}, {"eps": math.nan}):
+        with pytest.raises(ValueError, match="betas"):
+            make(**bad)
+    with pytest.raises(ValueError, match="step"):
+        make(step=-1)
+    for what in ("weight_decay", "lr_scale"):
+        for bad in (-0.1, math.nan, math.inf):
+            with pytest.raises(ValueError, match=what):
+                make(**{what: bad})
+        with pytest.raises(ValueError, match="one " + what):
+            make(**{what: [0.1, 0.2]})
+    with pytest.raises(TypeError, match="parameters"):
+        optim.AdamWPlan(_lists(dtype=torch.bfloat16), g)
+    with pytest.raises(TypeError, match="moments"):
+        make(exp_avg_sqs=_lists(dtype=torch.bfloat16))
+    with pytest.raises(TypeError, match="weights"):
+        make(weights=_lists(dtype=torch.float32))
+    for other in (_lists(shape=(8, 4)), [x.t().contiguous().t() for x in _lists()]):
+        with pytest.raises(ValueError, match="strides of their parameter"):
+            optim.AdamWPlan(p, other)
+        with pytest.raises(ValueError, match="strides of their parameter"):
+            make(exp_avgs=other)
+    with pytest.raises(ValueError, match="share memory"):
+        make(exp_avgs=g)
+    with pytest.raises(ValueError, match="share memory"):
+        make(exp_avgs=_lists(), exp_avg_sqs=[p[0]] + _lists(2))
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamWPlan([p[0], p[0]], g[:2])
+    with pytest.raises(RuntimeError, match="GPU"):                        # one gradient for two parameters is only read
+        optim.AdamWPlan(p, [g[0], g[0], g[1]])
+    with pytest.raises(RuntimeError, match="GPU"):
+        make(weights=[None, None, torch.zeros(4, 8, dtype=torch.bfloat16)], lr_scale=[1, 2.0, 3], weight_decay=0)
+
+
+def test_ranges():
+    a = torch.zeros(100)
+    ok = lambda w, r: optim._refuse_overlaps(w, r, "x")      # noqa: E731
+    ok([a[:10], a[10:20]], [a[20:30], a[25:40]])             # what is only read may overlap
+    ok([a[10:20], a[:0]], [a[:10], a[15:15], a[20:]])
+    for w, r in (([a[:10], a[9:20]], []), ([a[5:6]], [a[:100]]), ([a[:100]], [a[99:]]), ([a[3:7], a[3:7]], []),
+                 ([a[50:60]], [a[:55], a[2:4]]), ([a[:4], a[90:95]], [a[10:94]])):
+        with pytest.raises(ValueError, match="share memory"):
+            ok(w, r)
+
+
+def test_dense_and_self_overlap():
+    x = torch.zeros(4, 6, 5)
+    assert all(optim._is_dense(t) for t in (x, x.permute(2, 0, 1), x[1], x[:, :, :0], x[0, 0, 0], x[:1, 2:3].transpose(0, 1)))
+    assert not any(optim._is_dense(t) for t in (x[:, :3], x[..., ::2], x[:, 0], x[:1, :1].expand(4, 6, 5)))
+    for t in (x[:, :3], x[..., ::2], x.permute(1, 2, 0)[::3]):
+        optim._check_no_self_overlap(t, "x")
+    for t in (x[:1, :1].expand(4, 6, 5), torch.zeros(9).as_strided((3, 3), (2, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            optim._check_no_self_overlap(t, "x")
+
+
+def test_scalar_arguments():
+    dev = torch.device("cpu")
+    assert optim._scale_args(0.5, dev, "x") == (0.5, None) and optim._scale_args(2, dev, "x") == (2.0, None)
+    t = torch.ones(1)
+    assert optim._scale_args(t, dev, "x") == (1.0, t.data_ptr())
+    for bad in (-1.0, math.inf, math.nan, torch.ones(2), torch.ones((), dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            optim._scale_args(bad, dev, "x")
+
+
+def test_packed_floats_reach_the_descriptor():
+    """lr_scale and weight_decay travel as the two halves of one 8-byte word, lr_scale first, as wq_adamw_desc has them."""
+    word = np.array([[1.5, 0.25]], dtype=np.float32).view(np.int64)
+    assert [ctypes.c_float.from_buffer_copy(word.tobytes()[i:i + 4]).value for i in (0, 4)] == [1.5, 0.25]
