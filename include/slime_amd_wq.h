@@ -475,16 +475,17 @@ int wq_xxh3_128_grouped(const wq_xxh3_desc *descs, const int64_t *item_start, in
  * the AdamW update that folds the clip in and writes the low-precision weight (the tensors a weight sync then quantises).
  *
  * Gradients are bf16, fp16 or fp32 (any alignment that their elements have), every tensor a flat run of n elements.  The
- * launches read one descriptor per piece of at most WQ_GRAD_ITEM elements, made from per-tensor descriptors on the device
- * by wq_grad_make_items; the *_few forms take up to WQ_GRAD_FEW_MAX per-tensor descriptors from the HOST instead (read before
- * the call returns).  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
+ * launches read one descriptor per piece - WQ_GRAD_ITEM_BYTES of a gradient, WQ_ADAMW_ITEM elements of a parameter - made from
+ * per-tensor descriptors on the device by wq_grad_make_items; the *_few forms take up to WQ_GRAD_FEW_MAX per-tensor
+ * descriptors from the HOST instead (read before the call returns).  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
  * call and neither overflow nor lose small gradients (fp32 squares exactly).
  *
  * grad_scale (an inverse loss scale, 1 / number of tokens ...) multiplies every gradient; if grad_scale_dev is not NULL the
  * factor is grad_scale * grad_scale_dev[0], read on the device.  A norm is that of the scaled gradients.
  * coefficient = grad_scale * min(1, max_norm / (norm + 1e-6)), in fp32; a NaN norm makes it NaN, an infinite one 0 (NaN for
  * infinite max_norm), as torch.nn.utils.clip_grads_with_norm_ has it. */
-#define WQ_GRAD_ITEM 16384
+#define WQ_GRAD_ITEM_BYTES 16384
+#define WQ_ADAMW_ITEM 8192
 #define WQ_GRAD_FEW_MAX 64
 enum { WQ_NORM_2 = 0, WQ_NORM_INF = 1 };
 
@@ -511,7 +512,8 @@ typedef struct wq_adamw_desc {
 } wq_adamw_desc;
 
 /* `descs`: DEVICE array of n_desc wq_grad_desc (words = 4) or wq_adamw_desc (words = 8); item_start: DEVICE int64[n_desc+1],
- * exclusive prefix sum of ceil(n / WQ_GRAD_ITEM); items: DEVICE, n_items = item_start[n_desc] descriptors of the same kind. */
+ * exclusive prefix sum of the pieces of every tensor: ceil(n * bytes of an element of g / WQ_GRAD_ITEM_BYTES) for words = 4,
+ * ceil(n / WQ_ADAMW_ITEM) for words = 8.  items: DEVICE, n_items = item_start[n_desc] descriptors of the same kind. */
 int wq_grad_make_items(const void *descs, const int64_t *item_start, int n_desc, int64_t n_items, int words, void *items,
                        void *stream);
 

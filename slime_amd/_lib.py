@@ -28,7 +28,7 @@ INT4_DEQ_WORDS_PER_ITEM = 512
 BUCKET_COPY_MARK, BUCKET_COPY_BYTES = -1, 32768
 FP8_FEW_MAX = 4
 NORM_2, NORM_INF = 0, 1
-GRAD_ITEM, GRAD_FEW_MAX = 16384, 64
+GRAD_ITEM_BYTES, ADAMW_ITEM, GRAD_FEW_MAX = 16384, 8192, 64
 
 _i64, _int, _vp, _u32, _u64 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
 _f32, _f64 = ctypes.c_float, ctypes.c_double

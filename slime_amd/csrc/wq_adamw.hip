@@ -12,7 +12,10 @@
 
 namespace wq {
 
-constexpr int kAdamPiecesPerXcdRun = 32;
+constexpr int kAdamPart = 2048;                       // elements of a workgroup, a quarter of a piece
+constexpr int kAdamParts = kAdamItem / kAdamPart;
+constexpr int kAdamPartsPerXcdRun = 32;
+constexpr unsigned kAdamOccupancyPadBytes = 54000;    // unused dynamic LDS: at most 3 workgroups per CU
 
 struct AdamControl {       // at the start of the workspace, written anew by every step
     float coefficient;
@@ -45,7 +48,7 @@ __global__ __launch_bounds__(1024) void adamw_begin_kernel(const AdamBeginArgs a
     float norm = 0.0f;
     if (a.need_norm) {
         if (a.total_given) norm = ldg<float>(a.total_given);
-        else norm = NormAcc<NORM>::finish(fold_partials<NORM>(a.partials, a.n_partials, lds), scale);
+        else norm = NormAcc<NORM>::finish(fold_partials<NORM, 1024>(a.partials, a.n_partials, lds), scale);
     }
     if (threadIdx.x) return;
     if (a.need_norm && !a.total_given) stg<float>(a.total, norm);
@@ -82,23 +85,28 @@ __device__ __forceinline__ void adam_elem(float g, float& p, float& m, float& v,
     p = __builtin_fmaf(-s.step_size, m / denom, __builtin_fmaf(-s.decay, p, p));
 }
 
+struct AdamPart {
+    const char* g;
+    char *p, *m, *v, *o;
+    int n, g_dtype, out_dtype;
+};
+
 template <int G, int O>     // O < 0: no copy
-__device__ __forceinline__ void adam_piece(const wq_adamw_desc& d, const AdamConsts& k, const AdamStep& s)
+__device__ __forceinline__ void adam_part(const AdamPart& d, const AdamConsts& k, const AdamStep& s)
 {
-    const char* g = (const char*)d.g;
-    char *p = (char*)d.p, *m = (char*)d.m, *v = (char*)d.v, *o = (char*)d.out;
-    const int n = (int)d.n, whole = n / 4;
+    const int whole = d.n / 4;
     for (int i = threadIdx.x; i < whole; i += kGradThreads) {
+        const uint32_t at = (uint32_t)i * 16u;
         float gf[4];
         if constexpr (G == WQ_DTYPE_F32) {
-            const u32x4 w = ldg16(g + (size_t)i * 16);
+            const u32x4 w = ldg16_nt(d.g + at);
             gf[0] = u2f(w.x), gf[1] = u2f(w.y), gf[2] = u2f(w.z), gf[3] = u2f(w.w);
         } else {
-            const u32x2 w = ldg8(g + (size_t)i * 8);
+            const u32x2 w = ldg8_nt(d.g + at / 2);
             const f32x2 a = unpack2<G>(w.x), b = unpack2<G>(w.y);
             gf[0] = a.x, gf[1] = a.y, gf[2] = b.x, gf[3] = b.y;
         }
-        u32x4 pw = ldg16(p + (size_t)i * 16), mw = ldg16(m + (size_t)i * 16), vw = ldg16(v + (size_t)i * 16);
+        u32x4 pw = ldg16_nt(d.p + at), mw = ldg16_nt(d.m + at), vw = ldg16_nt(d.v + at);
         float pf[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -107,41 +115,46 @@ __device__ __forceinline__ void adam_piece(const wq_adamw_desc& d, const AdamCon
             adam_elem(gf[e], pf[e], mf, vf, k, s);
             pw[e] = f2u(pf[e]), mw[e] = f2u(mf), vw[e] = f2u(vf);
         }
-        stg16(p + (size_t)i * 16, pw);
-        stg16(m + (size_t)i * 16, mw);
-        stg16(v + (size_t)i * 16, vw);
-        if constexpr (O >= 0) stg8(o + (size_t)i * 8, (u32x2){pack2<O>(pf[0], pf[1]), pack2<O>(pf[2], pf[3])});
+        stg_nt_sc1<u32x4>(d.p + at, pw);
+        stg_nt_sc1<u32x4>(d.m + at, mw);
+        stg_nt_sc1<u32x4>(d.v + at, vw);
+        if constexpr (O >= 0) stg_nt_sc1<u32x2>(d.o + at / 2, (u32x2){pack2<O>(pf[0], pf[1]), pack2<O>(pf[2], pf[3])});
     }
     const int e = whole * 4 + threadIdx.x;
-    if (e < n) {
-        float pf = ldg<float>(p + (size_t)e * 4), mf = ldg<float>(m + (size_t)e * 4), vf = ldg<float>(v + (size_t)e * 4);
-        adam_elem(load_elem<G>(g, e), pf, mf, vf, k, s);
-        stg<float>(p + (size_t)e * 4, pf);
-        stg<float>(m + (size_t)e * 4, mf);
-        stg<float>(v + (size_t)e * 4, vf);
-        if constexpr (O >= 0) store_elem<O>(o, e, pf);
+    if (e < d.n) {
+        float pf = ldg<float>(d.p + (size_t)e * 4), mf = ldg<float>(d.m + (size_t)e * 4), vf = ldg<float>(d.v + (size_t)e * 4);
+        adam_elem(load_elem<G>(d.g, e), pf, mf, vf, k, s);
+        stg<float>(d.p + (size_t)e * 4, pf);
+        stg<float>(d.m + (size_t)e * 4, mf);
+        stg<float>(d.v + (size_t)e * 4, vf);
+        if constexpr (O >= 0) store_elem<O>(d.o, e, pf);
     }
 }
 template <int G>
-__device__ __forceinline__ void adam_piece_from(const wq_adamw_desc& d, const AdamConsts& k, const AdamStep& s)
+__device__ __forceinline__ void adam_part_from(const AdamPart& d, const AdamConsts& k, const AdamStep& s)
 {
-    if (!d.out) adam_piece<G, -1>(d, k, s);
-    else if (d.out_dtype == WQ_DTYPE_BF16) adam_piece<G, WQ_DTYPE_BF16>(d, k, s);
-    else adam_piece<G, WQ_DTYPE_F16>(d, k, s);
+    if (!d.o) adam_part<G, -1>(d, k, s);
+    else if (d.out_dtype == WQ_DTYPE_BF16) adam_part<G, WQ_DTYPE_BF16>(d, k, s);
+    else adam_part<G, WQ_DTYPE_F16>(d, k, s);
 }
 
-__global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc* items, const int64_t n_items, const AdamConsts k,
+__global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc* items, const int64_t n_parts, const AdamConsts k,
                                                             const AdamControl* control)
 {
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-    if (slot >= n_items) return;  // uniform per workgroup
+    if (slot >= n_parts) return;  // uniform per workgroup
     const AdamControl c = *control;
     if (c.skip) return;
-    const wq_adamw_desc d = items[xcd_chunked_item(slot, n_items, kAdamPiecesPerXcdRun)];
+    const int64_t part = xcd_chunked_item(slot, n_parts, kAdamPartsPerXcdRun);
+    const wq_adamw_desc d = items[part / kAdamParts];
+    const int at = (int)(part % kAdamParts) * kAdamPart, left = (int)d.n - at;
+    if (left <= 0) return;
+    const AdamPart a = {(const char*)d.g + at * dtype_bytes(d.g_dtype), (char*)(d.p + at), (char*)(d.m + at), (char*)(d.v + at),
+                        d.out ? (char*)d.out + at * 2 : nullptr, left < kAdamPart ? left : kAdamPart, d.g_dtype, d.out_dtype};
     const AdamStep s = {c.coefficient, c.lr * d.lr_scale * d.weight_decay, c.step_size * d.lr_scale, c.inv_sqrt_bc2};
-    if (d.g_dtype == WQ_DTYPE_BF16) adam_piece_from<WQ_DTYPE_BF16>(d, k, s);
-    else if (d.g_dtype == WQ_DTYPE_F16) adam_piece_from<WQ_DTYPE_F16>(d, k, s);
-    else adam_piece_from<WQ_DTYPE_F32>(d, k, s);
+    if (a.g_dtype == WQ_DTYPE_BF16) adam_part_from<WQ_DTYPE_BF16>(a, k, s);
+    else if (a.g_dtype == WQ_DTYPE_F16) adam_part_from<WQ_DTYPE_F16>(a, k, s);
+    else adam_part_from<WQ_DTYPE_F32>(a, k, s);
 }
 
 }  // namespace wq
@@ -158,8 +171,6 @@ WQ_EXPORT int wq_adamw_items(const wq_adamw_desc* items, int64_t n_items, const 
     if (need_norm && !h->total_given && !h->total) return WQ_ERR_NULL;
     hipStream_t st = (hipStream_t)stream;
     AdamBeginArgs a = {};
-    a.partials = partials_of(workspace);
-    a.n_partials = n_items;
     a.beta1 = h->beta1;
     a.beta2 = h->beta2;
     a.lr = h->lr;
@@ -172,13 +183,18 @@ WQ_EXPORT int wq_adamw_items(const wq_adamw_desc* items, int64_t n_items, const 
     a.max_norm = h->max_norm;
     a.need_norm = need_norm;
     a.skip_nonfinite = h->skip_nonfinite;
-    if (need_norm && !h->total_given) launch_norm_partials(TableSource{(const int64_t*)items, 8}, n_items, h->norm, partials_of(workspace), st);
+    if (need_norm && !h->total_given) {
+        const Partials p = launch_norm_partials(TableSource{(const int64_t*)items, 8}, n_items, h->norm, workspace, st);
+        a.partials = p.at;
+        a.n_partials = p.n;
+    }
     AdamControl* control = (AdamControl*)workspace;
     if (h->norm == WQ_NORM_2) adamw_begin_kernel<WQ_NORM_2><<<1, 1024, 0, st>>>(a, control);
     else adamw_begin_kernel<WQ_NORM_INF><<<1, 1024, 0, st>>>(a, control);
     if (n_items) {
         const AdamConsts k = {(float)h->beta1, (float)(1.0 - h->beta1), (float)h->beta2, (float)(1.0 - h->beta2), (float)h->eps};
-        adamw_kernel<<<grid_for_items(n_items), kGradThreads, 0, st>>>(items, n_items, k, control);
+        const int64_t parts = n_items * kAdamParts;
+        adamw_kernel<<<grid_for_items(parts), kGradThreads, kAdamOccupancyPadBytes, st>>>(items, parts, k, control);
     }
     WQ_LAUNCH_CHECK();
     return WQ_OK;

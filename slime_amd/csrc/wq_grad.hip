@@ -11,7 +11,13 @@
 
 namespace wq {
 
+// Both kernels: a workgroup takes 16 KiB of a gradient, four 16-byte loads per lane, all issued before the first use; an
+// unused dynamic LDS allocation caps the workgroups per CU.
+constexpr int kLoads = 4;
 constexpr int kNormPiecesPerXcdRun = 32;
+constexpr unsigned kNormOccupancyPadBytes = 27000;   // 6 workgroups per CU
+constexpr int kScalePiecesPerXcdRun = 32;
+constexpr unsigned kScaleOccupancyPadBytes = 54000;  // 3
 
 // ---- norm of a piece ------------------------------------------------------------------------------------------------
 template <int NORM, int D>
@@ -31,24 +37,26 @@ __device__ __forceinline__ void add_vec(typename NormAcc<NORM>::T& a, u32x4 v)
 template <int NORM, int D>
 __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece& p)
 {
-    constexpr int kVec = 16 / dtype_bytes(D), kLoads = 8;
+    constexpr int kVec = 16 / dtype_bytes(D), kBatch = kLoads * kGradThreads;
     typename NormAcc<NORM>::T a = NormAcc<NORM>::zero();
-    const int t = threadIdx.x;
-    if (p.n == kGradItem) {
+    const int t = threadIdx.x, whole = p.n / kVec;
+    for (int b = 0; b < whole; b += kBatch) {
+        u32x4 v[kLoads];
+        if (b + kBatch <= whole) {
 #pragma unroll
-        for (int b = 0; b < kGradItem / (kVec * kGradThreads * kLoads); ++b) {
-            u32x4 v[kLoads];
+            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(p.g + (size_t)(b + i * kGradThreads + t) * 16);
+        } else {  // lanes past the end load the last vector and count it as zeros
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = ldg16(p.g + (size_t)((b * kLoads + i) * kGradThreads + t) * 16);
+            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(p.g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) add_vec<NORM, D>(a, v[i]);
+            for (int i = 0; i < kLoads; ++i)
+                if (b + i * kGradThreads + t >= whole) v[i] = (u32x4){0u, 0u, 0u, 0u};
         }
-    } else {
-        const int whole = p.n / kVec;
-        for (int i = t; i < whole; i += kGradThreads) add_vec<NORM, D>(a, ldg16(p.g + (size_t)i * 16));
-        const int e = whole * kVec + t;
-        if (e < p.n) NormAcc<NORM>::add(a, load_elem<D>(p.g, e));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) add_vec<NORM, D>(a, v[i]);
     }
+    const int e = whole * kVec + t;
+    if (e < p.n) NormAcc<NORM>::add(a, load_elem<D>(p.g, e));
     return a;
 }
 
@@ -69,68 +77,95 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_partials_kernel(const 
     if (threadIdx.x == 0) stg<T>(partials + item * 8, a);
 }
 
+// one workgroup per kFoldGroup partials
+template <int NORM>
+__global__ __launch_bounds__(kGradThreads) void grad_norm_fold_kernel(const char* partials, const int64_t n, char* sums)
+{
+    typedef typename NormAcc<NORM>::T T;
+    __shared__ T lds[kGradThreads / 64];
+    const int64_t from = (int64_t)blockIdx.x * kFoldGroup, left = n - from;
+    const T a = fold_partials<NORM, kGradThreads>(partials + from * 8, left < kFoldGroup ? left : kFoldGroup, lds);
+    if (threadIdx.x == 0) stg<T>(sums + (int64_t)blockIdx.x * 8, a);
+}
+
 template <int NORM>
 __global__ __launch_bounds__(1024) void grad_norm_total_kernel(const char* partials, const int64_t n, const float scale,
                                                               const float* scale_dev, float* total)
 {
     typedef typename NormAcc<NORM>::T T;
     __shared__ T lds[16];
-    const T a = fold_partials<NORM>(partials, n, lds);
+    const T a = fold_partials<NORM, 1024>(partials, n, lds);
     if (threadIdx.x == 0) stg<float>(total, NormAcc<NORM>::finish(a, effective_scale(scale, scale_dev)));
 }
 
-// one wavefront per tensor
+// one workgroup per tensor
 template <int NORM>
-__global__ __launch_bounds__(64) void grad_norm_each_kernel(const char* partials, const int64_t* item_start, const float scale,
-                                                           const float* scale_dev, float* each)
+__global__ __launch_bounds__(kGradThreads) void grad_norm_each_kernel(const char* partials, const int64_t* item_start, const float scale,
+                                                                     const float* scale_dev, float* each)
 {
     typedef typename NormAcc<NORM>::T T;
+    __shared__ T lds[kGradThreads / 64];
     const int64_t from = item_start[blockIdx.x], to = item_start[blockIdx.x + 1];
-    T a = NormAcc<NORM>::zero();
-    for (int64_t i = from + threadIdx.x; i < to; i += 64) a = NormAcc<NORM>::join(a, ldg<T>(partials + i * 8));
-    a = wave_fold<NORM>(a);
+    const T a = fold_partials<NORM, kGradThreads>(partials + from * 8, to - from, lds);
     if (threadIdx.x == 0) stg<float>(each + blockIdx.x, NormAcc<NORM>::finish(a, effective_scale(scale, scale_dev)));
 }
 
 // ---- clip of a piece --------------------------------------------------------------------------------------------------
 // A lane takes the elements of one 16-byte access of the wider of the two types.
-template <int G, int O>
-__device__ __forceinline__ void piece_scale(const GradPiece& p, float c)
-{
-    constexpr bool kWide = G == WQ_DTYPE_F32 || O == WQ_DTYPE_F32;
-    constexpr int kElems = kWide ? 4 : 8;
-    const int whole = p.n / kElems;
-    for (int i = threadIdx.x; i < whole; i += kGradThreads) {
-        float f[kElems];
-        if constexpr (G == WQ_DTYPE_F32) {
-            const u32x4 v = ldg16(p.g + (size_t)i * 16);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = u2f(v[k]) * c;
+template <int G, int O> struct ScaleVec {
+    static constexpr int kElems = G == WQ_DTYPE_F32 || O == WQ_DTYPE_F32 ? 4 : 8;
+    static constexpr int kIn = kElems * dtype_bytes(G), kOut = kElems * dtype_bytes(O);
+    uint32_t w[kIn / 4];
+    __device__ __forceinline__ void load(const char* p)
+    {
+        if constexpr (kIn == 16) {
+            const u32x4 v = ldg16_nt(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         } else {
-            uint32_t w[kElems / 2];
-            if constexpr (kElems == 8) {
-                const u32x4 v = ldg16(p.g + (size_t)i * 16);
-                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else {
-                const u32x2 v = ldg8(p.g + (size_t)i * 8);
-                w[0] = v.x, w[1] = v.y;
-            }
+            const u32x2 v = ldg8_nt(p);
+            w[0] = v.x, w[1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void scale_and_store(char* p, float c) const
+    {
+        float f[kElems];
 #pragma unroll
-            for (int k = 0; k < kElems / 2; ++k) {
+        for (int k = 0; k < kIn / 4; ++k) {
+            if constexpr (G == WQ_DTYPE_F32) {
+                f[k] = u2f(w[k]) * c;
+            } else {
                 const f32x2 x = unpack2<G>(w[k]);
                 f[2 * k] = x.x * c;
                 f[2 * k + 1] = x.y * c;
             }
         }
-        if constexpr (O == WQ_DTYPE_F32) {
-            stg16(p.out + (size_t)i * 16, (u32x4){f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])});
-        } else if constexpr (kElems == 8) {
-            stg16(p.out + (size_t)i * 16, (u32x4){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3]), pack2<O>(f[4], f[5]), pack2<O>(f[6], f[7])});
-        } else {
-            stg8(p.out + (size_t)i * 8, (u32x2){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3])});
+        if constexpr (O == WQ_DTYPE_F32) stg_nt_sc1<u32x4>(p, (u32x4){f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])});
+        else if constexpr (kElems == 4) stg_nt_sc1<u32x2>(p, (u32x2){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3])});
+        else stg_nt_sc1<u32x4>(p, (u32x4){pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3]), pack2<O>(f[4], f[5]), pack2<O>(f[6], f[7])});
+    }
+};
+template <int G, int O>
+__device__ __forceinline__ void piece_scale(const GradPiece& p, float c)
+{
+    typedef ScaleVec<G, O> Vec;
+    constexpr int kBatch = kLoads * kGradThreads;
+    const int t = threadIdx.x, whole = p.n / Vec::kElems;
+    for (int b = 0; b < whole; b += kBatch) {
+        Vec v[kLoads];
+        if (b + kBatch <= whole) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i].load(p.g + (size_t)(b + i * kGradThreads + t) * Vec::kIn);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i].scale_and_store(p.out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
+        } else {  // lanes past the end load the last vector (in place perhaps as its owner stores it) and drop it
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i].load(p.g + (size_t)min(b + i * kGradThreads + t, whole - 1) * Vec::kIn);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (b + i * kGradThreads + t < whole) v[i].scale_and_store(p.out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
         }
     }
-    const int e = whole * kElems + threadIdx.x;
+    const int e = whole * Vec::kElems + t;
     if (e < p.n) store_elem<O>(p.out, e, load_elem<G>(p.g, e) * c);
 }
 template <int G>
@@ -148,7 +183,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source s
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
     if (slot >= n_items) return;  // uniform per workgroup
     const float c = clip_coefficient(ldg<float>(total), max_norm, effective_scale(scale, scale_dev));
-    const GradPiece p = src.piece(xcd_chunked_item(slot, n_items, kNormPiecesPerXcdRun));
+    // last piece first: what the norm read last is what a cache still holds
+    const GradPiece p = src.piece(n_items - 1 - xcd_chunked_item(slot, n_items, kScalePiecesPerXcdRun));
     if (c == 1.0f && p.out == p.g) return;
     if (p.g_dtype == WQ_DTYPE_BF16) piece_scale_from<WQ_DTYPE_BF16>(p, c);
     else if (p.g_dtype == WQ_DTYPE_F16) piece_scale_from<WQ_DTYPE_F16>(p, c);
@@ -164,11 +200,12 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
     const int i = find_owner(item_start, n_desc, t, n_items);
     const int64_t* d = descs + (int64_t)i * words;
     int64_t* o = items + t * words;
-    const int64_t at = (t - item_start[i]) * kGradItem, left = d[2] - at;
     const int g_dtype = (int)(uint32_t)d[3], out_dtype = (int)(uint32_t)((uint64_t)d[3] >> 32);
+    const int item = words == 4 ? grad_item(g_dtype) : kAdamItem;
+    const int64_t at = (t - item_start[i]) * item, left = d[2] - at;
     o[0] = d[0] + at * dtype_bytes(g_dtype);
     o[1] = d[1] ? d[1] + at * dtype_bytes(out_dtype) : 0;
-    o[2] = left < kGradItem ? left : kGradItem;
+    o[2] = left < item ? left : item;
     o[3] = d[3];
     if (words == 8) {
         o[4] = d[4] + at * 4;
@@ -178,27 +215,35 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
     }
 }
 
-template <typename Source>
-static void launch_partials(const Source& src, int64_t n_items, int norm, void* partials, hipStream_t st)
+template <int NORM, typename Source>
+static Partials launch_partials(const Source& src, int64_t n_items, void* workspace, hipStream_t st)
 {
-    if (n_items == 0) return;
-    const dim3 g = grid_for_items(n_items);
-    if (norm == WQ_NORM_2) grad_norm_partials_kernel<WQ_NORM_2><<<g, kGradThreads, 0, st>>>(src, n_items, (char*)partials);
-    else grad_norm_partials_kernel<WQ_NORM_INF><<<g, kGradThreads, 0, st>>>(src, n_items, (char*)partials);
+    char* partials = partials_of(workspace);
+    if (n_items) grad_norm_partials_kernel<NORM><<<grid_for_items(n_items), kGradThreads, kNormOccupancyPadBytes, st>>>(src, n_items, partials);
+    if (n_items <= kFoldDirect) return {partials, n_items};
+    const int64_t groups = cdiv64(n_items, kFoldGroup);
+    char* sums = partials + n_items * 8;
+    grad_norm_fold_kernel<NORM><<<(unsigned)groups, kGradThreads, 0, st>>>(partials, n_items, sums);
+    return {sums, groups};
 }
-void launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* partials, hipStream_t st)
+Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st)
 {
-    launch_partials(src, n_items, norm, partials, st);
+    return norm == WQ_NORM_2 ? launch_partials<WQ_NORM_2>(src, n_items, workspace, st) : launch_partials<WQ_NORM_INF>(src, n_items, workspace, st);
 }
 
+template <int NORM, typename Source>
+static void launch_norm_kind(const Source& src, int64_t n_items, float scale, const float* scale_dev, void* workspace, float* total,
+                             hipStream_t st)
+{
+    const Partials p = launch_partials<NORM>(src, n_items, workspace, st);
+    grad_norm_total_kernel<NORM><<<1, 1024, 0, st>>>(p.at, p.n, scale, scale_dev, total);
+}
 template <typename Source>
 static void launch_norm(const Source& src, int64_t n_items, int norm, float scale, const float* scale_dev, void* workspace,
                         float* total, hipStream_t st)
 {
-    char* partials = partials_of(workspace);
-    launch_partials(src, n_items, norm, partials, st);
-    if (norm == WQ_NORM_2) grad_norm_total_kernel<WQ_NORM_2><<<1, 1024, 0, st>>>(partials, n_items, scale, scale_dev, total);
-    else grad_norm_total_kernel<WQ_NORM_INF><<<1, 1024, 0, st>>>(partials, n_items, scale, scale_dev, total);
+    if (norm == WQ_NORM_2) launch_norm_kind<WQ_NORM_2>(src, n_items, scale, scale_dev, workspace, total, st);
+    else launch_norm_kind<WQ_NORM_INF>(src, n_items, scale, scale_dev, workspace, total, st);
 }
 template <typename Source>
 static void launch_clip(const Source& src, int64_t n_items, int norm, float max_norm, float scale, const float* scale_dev,
@@ -206,7 +251,8 @@ static void launch_clip(const Source& src, int64_t n_items, int norm, float max_
 {
     if (!given) launch_norm(src, n_items, norm, scale, scale_dev, workspace, total, st);
     if (n_items == 0) return;
-    grad_scale_kernel<<<grid_for_items(n_items), kGradThreads, 0, st>>>(src, n_items, given ? given : total, max_norm, scale, scale_dev);
+    grad_scale_kernel<<<grid_for_items(n_items), kGradThreads, kScaleOccupancyPadBytes, st>>>(src, n_items, given ? given : total,
+                                                                                              max_norm, scale, scale_dev);
 }
 
 static bool grad_dtype_ok(int d) { return d == WQ_DTYPE_BF16 || d == WQ_DTYPE_F16 || d == WQ_DTYPE_F32; }
@@ -225,7 +271,7 @@ static int64_t few_source(const wq_grad_desc* descs, int n_desc, bool with_out, 
         if (!descs[i].g || (with_out && !descs[i].out)) return WQ_ERR_NULL;
         src->d[k] = descs[i];
         src->start[k++] = items;
-        items += cdiv64(descs[i].n, kGradItem);
+        items += cdiv64(descs[i].n, grad_item(descs[i].g_dtype));
     }
     src->start[k] = items;
     src->n_desc = k;
@@ -236,7 +282,7 @@ static int64_t few_source(const wq_grad_desc* descs, int n_desc, bool with_out, 
 
 using namespace wq;
 
-WQ_EXPORT int64_t wq_grad_workspace_bytes(int64_t n_items) { return n_items < 0 ? 0 : kGradControlBytes + n_items * 8; }
+WQ_EXPORT int64_t wq_grad_workspace_bytes(int64_t n_items) { return n_items < 0 ? 0 : kGradControlBytes + (n_items + cdiv64(n_items, kFoldGroup)) * 8; }
 
 WQ_EXPORT int wq_grad_make_items(const void* descs, const int64_t* item_start, int n_desc, int64_t n_items, int words, void* items,
                                  void* stream)
@@ -262,8 +308,8 @@ WQ_EXPORT int wq_grad_norm_items(const void* items, int64_t n_items, int words, 
     launch_norm(TableSource{(const int64_t*)items, words}, n_items, norm, grad_scale, grad_scale_dev, workspace, total, st);
     if (each && n_desc) {
         const char* partials = partials_of(workspace);
-        if (norm == WQ_NORM_2) grad_norm_each_kernel<WQ_NORM_2><<<n_desc, 64, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
-        else grad_norm_each_kernel<WQ_NORM_INF><<<n_desc, 64, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
+        if (norm == WQ_NORM_2) grad_norm_each_kernel<WQ_NORM_2><<<n_desc, kGradThreads, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
+        else grad_norm_each_kernel<WQ_NORM_INF><<<n_desc, kGradThreads, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
     }
     WQ_LAUNCH_CHECK();
     return WQ_OK;

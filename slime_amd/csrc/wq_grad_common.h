@@ -11,18 +11,18 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kGradThreads = 256;
-constexpr int kGradItem = WQ_GRAD_ITEM;
+constexpr int kAdamItem = WQ_ADAMW_ITEM;
 
 // 16- and 8-byte accesses of streams whose elements have their own alignment only (a tensor inside a packed buffer starts
 // anywhere): gfx950's global accesses take any address, the type says so to the compiler.
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
-__device__ __forceinline__ u32x4 ldg16(const char* p) { return *(const WQ_GLOBAL u32x4_a2*)p; }
-__device__ __forceinline__ u32x2 ldg8(const char* p) { return *(const WQ_GLOBAL u32x2_a2*)p; }
-__device__ __forceinline__ void stg16(char* p, u32x4 v) { *(WQ_GLOBAL u32x4_a2*)p = v; }
-__device__ __forceinline__ void stg8(char* p, u32x2 v) { *(WQ_GLOBAL u32x2_a2*)p = v; }
+__device__ __forceinline__ u32x4 ldg16_nt(const char* p) { return __builtin_nontemporal_load((const WQ_GLOBAL u32x4_a2*)p); }
+__device__ __forceinline__ u32x2 ldg8_nt(const char* p) { return __builtin_nontemporal_load((const WQ_GLOBAL u32x2_a2*)p); }
 
-constexpr int dtype_bytes(int d) { return d == WQ_DTYPE_F32 ? 4 : 2; }
+__host__ __device__ constexpr int dtype_bytes(int d) { return d == WQ_DTYPE_F32 ? 4 : 2; }
+// elements of a gradient piece
+__host__ __device__ constexpr int grad_item(int d) { return WQ_GRAD_ITEM_BYTES / dtype_bytes(d); }
 
 template <int D>
 __device__ __forceinline__ float load_elem(const char* p, int i)
@@ -85,10 +85,10 @@ struct FewSource {
             const int mid = (lo + hi) >> 1;
             if (start[mid] <= t) lo = mid; else hi = mid;
         }
-        const int64_t at = (t - start[lo]) * kGradItem;
-        const int64_t left = d[lo].n - at;
+        const int item = grad_item(d[lo].g_dtype);
+        const int64_t at = (t - start[lo]) * item, left = d[lo].n - at;
         return {(const char*)d[lo].g + at * dtype_bytes(d[lo].g_dtype), (char*)d[lo].out + at * dtype_bytes(d[lo].out_dtype),
-                (int)(left < kGradItem ? left : kGradItem), d[lo].g_dtype, d[lo].out_dtype};
+                (int)(left < item ? left : item), d[lo].g_dtype, d[lo].out_dtype};
     }
 };
 
@@ -142,14 +142,24 @@ __device__ __forceinline__ typename NormAcc<NORM>::T block_fold(typename NormAcc
     return a;
 }
 
-// The fold of all partials by one workgroup of 1024, in an order that depends on their number only.
-template <int NORM>
-__device__ __forceinline__ typename NormAcc<NORM>::T fold_partials(const void* partials, int64_t n, typename NormAcc<NORM>::T* lds)
+// The fold of n values by one workgroup of THREADS, in an order that depends on n only; eight loads in flight per lane.
+template <int NORM, int THREADS>
+__device__ __forceinline__ typename NormAcc<NORM>::T fold_partials(const char* partials, int64_t n, typename NormAcc<NORM>::T* lds)
 {
     typedef typename NormAcc<NORM>::T T;
     T a = NormAcc<NORM>::zero();
-    for (int64_t i = threadIdx.x; i < n; i += 1024) a = NormAcc<NORM>::join(a, ldg<T>((const char*)partials + i * 8));
-    return block_fold<NORM, 16>(a, lds);
+    for (int64_t i = threadIdx.x; i < n; i += 8 * THREADS) {
+        T v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t k = i + u * THREADS;
+            v[u] = ldg<T>(partials + (k < n ? k : n - 1) * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i + u * THREADS < n) a = NormAcc<NORM>::join(a, v[u]);
+    }
+    return block_fold<NORM, THREADS / 64>(a, lds);
 }
 
 __device__ __forceinline__ float effective_scale(float scale, const float* dev) { return dev ? scale * ldg<float>(dev) : scale; }
@@ -159,11 +169,17 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm, fl
     return (c > 1.0f ? 1.0f : c) * scale;      // NaN stays NaN
 }
 
-// workspace: 64 bytes of AdamW's per-step values, then the partials
+// workspace: 64 bytes of AdamW's per-step values, one partial per piece, and the sums of kFoldGroup partials each that long
+// lists fold first: one workgroup folds kFoldGroup partials in about 2 us, and a whole model's 900 000 would take it 60.
 constexpr int64_t kGradControlBytes = 64;
+constexpr int64_t kFoldGroup = 4096, kFoldDirect = 4 * kFoldGroup;
 inline char* partials_of(void* workspace) { return (char*)workspace + kGradControlBytes; }
+struct Partials {
+    const char* at;
+    int64_t n;
+};
 
-// wq_grad.hip: one partial per piece
-void launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* partials, hipStream_t st);
+// wq_grad.hip: one partial per piece, folded to at most kFoldDirect (or n_items / kFoldGroup) values for a last fold
+Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st);
 
 }  // namespace wq

@@ -139,8 +139,8 @@ def _bump(tensors) -> None:
         torch.autograd.graph.increment_version(tensors)
 
 
-def _pieces(n: int) -> int:
-    return -(-n // _lib.GRAD_ITEM)
+def _pieces(t) -> int:
+    return -(-t.numel() * t.element_size() // _lib.GRAD_ITEM_BYTES)
 
 
 def _workspace(n_items: int, device) -> torch.Tensor:
@@ -156,7 +156,11 @@ def _item_table(rows: np.ndarray, device, what: str, wait: bool):
     """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
     of the tensors in it).  Without ``wait`` the upload goes through pinned memory and the host goes on."""
     starts = np.zeros(len(rows) + 1, dtype=np.int64)
-    np.cumsum(-(-rows[:, 2] // _lib.GRAD_ITEM), out=starts[1:])
+    if rows.shape[1] == 8:
+        per = _lib.ADAMW_ITEM
+    else:
+        per = np.where(rows[:, 3] & 0xFFFFFFFF == _lib.DTYPE_F32, _lib.GRAD_ITEM_BYTES // 4, _lib.GRAD_ITEM_BYTES // 2)
+    np.cumsum(-(-rows[:, 2] // per), out=starts[1:])
     host = torch.from_numpy(np.concatenate([rows.reshape(-1), starts]))
     if wait:
         table = host.to(device)
@@ -393,7 +397,7 @@ def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
 def _total_norm(tensors, device, norm: int, what: str) -> torch.Tensor:
     dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
     total = torch.empty((), dtype=torch.float32, device=device)
-    ws = _workspace(sum(_pieces(t.numel()) for t in dense), device)
+    ws = _workspace(sum(_pieces(t) for t in dense), device)
     _call(dense, device, "wq_grad_norm_few", "wq_grad_norm_items", what, (norm, 1.0, ws.data_ptr(), total.data_ptr()),
           lambda items, starts, n_items, n: (items, n_items, 4, starts, n, norm, 1.0, None, ws.data_ptr(), total.data_ptr(), None))
     return total
@@ -426,7 +430,7 @@ def _clip(grads, max_norm: float, norm: int, total_norm, what: str) -> torch.Ten
     work = dense + [c for _, c in copies]
     if total_norm is None:
         total = torch.empty((), dtype=torch.float32, device=device)
-        ws, given = _workspace(sum(_pieces(g.numel()) for g in work), device).data_ptr(), None
+        ws, given = _workspace(sum(_pieces(g) for g in work), device).data_ptr(), None
     else:
         total = total_norm.detach().to(device=device, dtype=torch.float32)
         ws, given = None, total.data_ptr()

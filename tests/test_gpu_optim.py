@@ -548,4 +548,4 @@ def test_a_list_of_more_than_four_gigabytes(cuda):
 
 
 def test_abi_constants_match(cuda):
-    assert _lib.GRAD_ITEM == ITEM
+    assert _lib.GRAD_ITEM_BYTES == ITEM and 2 * _lib.ADAMW_ITEM == ITEM
