@@ -512,8 +512,11 @@ typedef struct wq_adamw_desc {
 } wq_adamw_desc;
 
 /* `descs`: DEVICE array of n_desc wq_grad_desc (words = 4) or wq_adamw_desc (words = 8); item_start: DEVICE int64[n_desc+1],
- * exclusive prefix sum of the pieces of every tensor: ceil(n * bytes of an element of g / WQ_GRAD_ITEM_BYTES) for words = 4,
- * ceil(n / WQ_ADAMW_ITEM) for words = 8.  items: DEVICE, n_items = item_start[n_desc] descriptors of the same kind. */
+ * exclusive prefix sum of the pieces of every tensor; items: DEVICE, n_items = item_start[n_desc] descriptors of the same kind.
+ * Pieces end at 128-byte lines: ceil((n + phase) / item) of them for n > 0, where
+ *   words = 4: item = WQ_GRAD_ITEM_BYTES / bytes of an element of g; phase = elements of `out` behind the last 128-byte line
+ *              before it if out is given and its elements are no smaller than g's, else those of g;
+ *   words = 8: item = WQ_ADAMW_ITEM, phase that of p. */
 int wq_grad_make_items(const void *descs, const int64_t *item_start, int n_desc, int64_t n_items, int words, void *items,
                        void *stream);
 

@@ -94,19 +94,21 @@ struct AdamPart {
 template <int G, int O>     // O < 0: no copy
 __device__ __forceinline__ void adam_part(const AdamPart& d, const AdamConsts& k, const AdamStep& s)
 {
-    const int whole = d.n / 4;
+    const int head = head_of(d.p, 4, d.n), whole = (d.n - head) / 4;
+    const char* g = d.g + head * dtype_bytes(G);
+    char *p = d.p + head * 4, *m = d.m + head * 4, *v = d.v + head * 4, *o = d.o + head * 2;
     for (int i = threadIdx.x; i < whole; i += kGradThreads) {
         const uint32_t at = (uint32_t)i * 16u;
         float gf[4];
         if constexpr (G == WQ_DTYPE_F32) {
-            const u32x4 w = ldg16_nt(d.g + at);
+            const u32x4 w = ldg16_nt(g + at);
             gf[0] = u2f(w.x), gf[1] = u2f(w.y), gf[2] = u2f(w.z), gf[3] = u2f(w.w);
         } else {
-            const u32x2 w = ldg8_nt(d.g + at / 2);
+            const u32x2 w = ldg8_nt(g + at / 2);
             const f32x2 a = unpack2<G>(w.x), b = unpack2<G>(w.y);
             gf[0] = a.x, gf[1] = a.y, gf[2] = b.x, gf[3] = b.y;
         }
-        u32x4 pw = ldg16_nt(d.p + at), mw = ldg16_nt(d.m + at), vw = ldg16_nt(d.v + at);
+        u32x4 pw = ldg16_nt(p + at), mw = ldg16_nt(m + at), vw = ldg16_nt(v + at);
         float pf[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -115,12 +117,14 @@ __device__ __forceinline__ void adam_part(const AdamPart& d, const AdamConsts& k
             adam_elem(gf[e], pf[e], mf, vf, k, s);
             pw[e] = f2u(pf[e]), mw[e] = f2u(mf), vw[e] = f2u(vf);
         }
-        stg_nt_sc1<u32x4>(d.p + at, pw);
-        stg_nt_sc1<u32x4>(d.m + at, mw);
-        stg_nt_sc1<u32x4>(d.v + at, vw);
-        if constexpr (O >= 0) stg_nt_sc1<u32x2>(d.o + at / 2, (u32x2){pack2<O>(pf[0], pf[1]), pack2<O>(pf[2], pf[3])});
+        stg_nt_sc1<u32x4>(p + at, pw);
+        stg_nt_sc1<u32x4>(m + at, mw);
+        stg_nt_sc1<u32x4>(v + at, vw);
+        if constexpr (O >= 0) stg_nt_sc1<u32x2>(o + at / 2, (u32x2){pack2<O>(pf[0], pf[1]), pack2<O>(pf[2], pf[3])});
     }
-    const int e = whole * 4 + threadIdx.x;
+    // before the first boundary and behind the last vector: a lane per element
+    const int t = threadIdx.x, behind = head + whole * 4;
+    const int e = t < head ? t : behind + t - head;
     if (e < d.n) {
         float pf = ldg<float>(d.p + (size_t)e * 4), mf = ldg<float>(d.m + (size_t)e * 4), vf = ldg<float>(d.v + (size_t)e * 4);
         adam_elem(load_elem<G>(d.g, e), pf, mf, vf, k, s);
@@ -147,10 +151,11 @@ __global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc
     if (c.skip) return;
     const int64_t part = xcd_chunked_item(slot, n_parts, kAdamPartsPerXcdRun);
     const wq_adamw_desc d = items[part / kAdamParts];
-    const int at = (int)(part % kAdamParts) * kAdamPart, left = (int)d.n - at;
-    if (left <= 0) return;
+    const Run r = run_of(part % kAdamParts, d.n, kAdamPart, phase_of(d.p, 4));
+    if (r.n <= 0) return;
+    const int at = (int)r.at;
     const AdamPart a = {(const char*)d.g + at * dtype_bytes(d.g_dtype), (char*)(d.p + at), (char*)(d.m + at), (char*)(d.v + at),
-                        d.out ? (char*)d.out + at * 2 : nullptr, left < kAdamPart ? left : kAdamPart, d.g_dtype, d.out_dtype};
+                        d.out ? (char*)d.out + at * 2 : nullptr, r.n, d.g_dtype, d.out_dtype};
     const AdamStep s = {c.coefficient, c.lr * d.lr_scale * d.weight_decay, c.step_size * d.lr_scale, c.inv_sqrt_bc2};
     if (a.g_dtype == WQ_DTYPE_BF16) adam_part_from<WQ_DTYPE_BF16>(a, k, s);
     else if (a.g_dtype == WQ_DTYPE_F16) adam_part_from<WQ_DTYPE_F16>(a, k, s);

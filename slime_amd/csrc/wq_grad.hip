@@ -39,15 +39,16 @@ __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece&
 {
     constexpr int kVec = 16 / dtype_bytes(D), kBatch = kLoads * kGradThreads;
     typename NormAcc<NORM>::T a = NormAcc<NORM>::zero();
-    const int t = threadIdx.x, whole = p.n / kVec;
+    const int t = threadIdx.x, head = head_of(p.g, dtype_bytes(D), p.n), whole = (p.n - head) / kVec;
+    const char* g = p.g + head * dtype_bytes(D);
     for (int b = 0; b < whole; b += kBatch) {
         u32x4 v[kLoads];
         if (b + kBatch <= whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(p.g + (size_t)(b + i * kGradThreads + t) * 16);
+            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(g + (size_t)(b + i * kGradThreads + t) * 16);
         } else {  // lanes past the end load the last vector and count it as zeros
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(p.g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
+            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
                 if (b + i * kGradThreads + t >= whole) v[i] = (u32x4){0u, 0u, 0u, 0u};
@@ -55,8 +56,9 @@ __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece&
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) add_vec<NORM, D>(a, v[i]);
     }
+    if (t < head) NormAcc<NORM>::add(a, load_elem<D>(p.g, t));
     const int e = whole * kVec + t;
-    if (e < p.n) NormAcc<NORM>::add(a, load_elem<D>(p.g, e));
+    if (e < p.n - head) NormAcc<NORM>::add(a, load_elem<D>(g, e));
     return a;
 }
 
@@ -149,24 +151,28 @@ __device__ __forceinline__ void piece_scale(const GradPiece& p, float c)
 {
     typedef ScaleVec<G, O> Vec;
     constexpr int kBatch = kLoads * kGradThreads;
-    const int t = threadIdx.x, whole = p.n / Vec::kElems;
+    constexpr int kG = dtype_bytes(G), kO = dtype_bytes(O);
+    const int t = threadIdx.x, head = kO >= kG ? head_of(p.out, kO, p.n) : head_of(p.g, kG, p.n), n = p.n - head, whole = n / Vec::kElems;
+    const char* g = p.g + head * kG;
+    char* out = p.out + head * kO;
     for (int b = 0; b < whole; b += kBatch) {
         Vec v[kLoads];
         if (b + kBatch <= whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].load(p.g + (size_t)(b + i * kGradThreads + t) * Vec::kIn);
+            for (int i = 0; i < kLoads; ++i) v[i].load(g + (size_t)(b + i * kGradThreads + t) * Vec::kIn);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].scale_and_store(p.out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
+            for (int i = 0; i < kLoads; ++i) v[i].scale_and_store(out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
         } else {  // lanes past the end load the last vector (in place perhaps as its owner stores it) and drop it
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].load(p.g + (size_t)min(b + i * kGradThreads + t, whole - 1) * Vec::kIn);
+            for (int i = 0; i < kLoads; ++i) v[i].load(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * Vec::kIn);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (b + i * kGradThreads + t < whole) v[i].scale_and_store(p.out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
+                if (b + i * kGradThreads + t < whole) v[i].scale_and_store(out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
         }
     }
     const int e = whole * Vec::kElems + t;
-    if (e < p.n) store_elem<O>(p.out, e, load_elem<G>(p.g, e) * c);
+    if (e < n) store_elem<O>(out, e, load_elem<G>(g, e) * c);
+    if (t < head) store_elem<O>(p.out, t, load_elem<G>(p.g, t) * c);
 }
 template <int G>
 __device__ __forceinline__ void piece_scale_from(const GradPiece& p, float c)
@@ -192,25 +198,38 @@ __global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source s
 }
 
 // ---- per-tensor descriptors -> one per piece ----------------------------------------------------------------------------
+// Hides that a per-lane factor is a power of two.  From "times 4096 or 8192" the compiler makes a 64-bit shift by a VGPR, and
+// on gfx950 that shift goes wrong now and then if the amount is in the last VGPR the kernel has (100 of 13 863 wavefronts
+// left their value unshifted): as a number it multiplies.
+__device__ __forceinline__ int plain_factor(int x)
+{
+    asm("" : "+v"(x));
+    return x;
+}
 __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* descs, const int64_t* __restrict__ item_start,
                                                              const int n_desc, const int64_t n_items, const int words, int64_t* items)
 {
     const int64_t t = ((int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x) * 256 + threadIdx.x;
     if (t >= n_items) return;
-    const int i = find_owner(item_start, n_desc, t, n_items);
+    int i = 0, hi = n_desc;
+    while (hi - i > 1) {  // item_start[i] <= t < item_start[hi]
+        const int mid = (i + hi) >> 1;
+        if (item_start[mid] <= t) i = mid; else hi = mid;
+    }
     const int64_t* d = descs + (int64_t)i * words;
     int64_t* o = items + t * words;
     const int g_dtype = (int)(uint32_t)d[3], out_dtype = (int)(uint32_t)((uint64_t)d[3] >> 32);
-    const int item = words == 4 ? grad_item(g_dtype) : kAdamItem;
-    const int64_t at = (t - item_start[i]) * item, left = d[2] - at;
-    o[0] = d[0] + at * dtype_bytes(g_dtype);
-    o[1] = d[1] ? d[1] + at * dtype_bytes(out_dtype) : 0;
-    o[2] = left < item ? left : item;
+    const int g_bytes = plain_factor(dtype_bytes(g_dtype)), out_bytes = plain_factor(dtype_bytes(out_dtype));
+    const Run r = words == 4 ? run_of(t - item_start[i], d[2], plain_factor(grad_item(g_dtype)), grad_phase(*(const wq_grad_desc*)d))
+                             : run_of(t - item_start[i], d[2], kAdamItem, phase_of((const void*)d[4], 4));
+    o[0] = d[0] + r.at * g_bytes;
+    o[1] = d[1] ? d[1] + r.at * out_bytes : 0;
+    o[2] = r.n;
     o[3] = d[3];
     if (words == 8) {
-        o[4] = d[4] + at * 4;
-        o[5] = d[5] + at * 4;
-        o[6] = d[6] + at * 4;
+        o[4] = d[4] + r.at * 4;
+        o[5] = d[5] + r.at * 4;
+        o[6] = d[6] + r.at * 4;
         o[7] = d[7];
     }
 }
@@ -270,8 +289,9 @@ static int64_t few_source(const wq_grad_desc* descs, int n_desc, bool with_out, 
         if (descs[i].n == 0) continue;
         if (!descs[i].g || (with_out && !descs[i].out)) return WQ_ERR_NULL;
         src->d[k] = descs[i];
+        if (!with_out) src->d[k].out = nullptr;
         src->start[k++] = items;
-        items += cdiv64(descs[i].n, grad_item(descs[i].g_dtype));
+        items += pieces_of(descs[i].n, grad_item(descs[i].g_dtype), grad_phase(src->d[k - 1]));
     }
     src->start[k] = items;
     src->n_desc = k;

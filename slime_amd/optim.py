@@ -139,8 +139,9 @@ def _bump(tensors) -> None:
         torch.autograd.graph.increment_version(tensors)
 
 
-def _pieces(t) -> int:
-    return -(-t.numel() * t.element_size() // _lib.GRAD_ITEM_BYTES)
+def _most_pieces(t) -> int:
+    """At least the number of pieces of a gradient, wherever it starts."""
+    return t.numel() * t.element_size() // _lib.GRAD_ITEM_BYTES + 2
 
 
 def _workspace(n_items: int, device) -> torch.Tensor:
@@ -152,15 +153,22 @@ def _grad_row(g, out=None):
     return [g.data_ptr(), out.data_ptr(), g.numel(), _DTYPES[g.dtype] | _DTYPES[out.dtype] << 32]
 
 
+def _cuts(rows: np.ndarray):
+    """-> (elements of a piece, elements by which the first is shorter) per row: pieces are cut at 128-byte lines of the fp32
+    weight of an update, of the wider stream of a clip."""
+    if rows.shape[1] == 8:
+        return _lib.ADAMW_ITEM, rows[:, 4] % 128 // 4
+    g, o = (np.where(d == _lib.DTYPE_F32, 4, 2) for d in (rows[:, 3] & 0xFFFFFFFF, rows[:, 3] >> 32))
+    return _lib.GRAD_ITEM_BYTES // g, np.where((rows[:, 1] != 0) & (o >= g), rows[:, 1] % 128 // o, rows[:, 0] % 128 // g)
+
+
 def _item_table(rows: np.ndarray, device, what: str, wait: bool):
     """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
     of the tensors in it).  Without ``wait`` the upload goes through pinned memory and the host goes on."""
     starts = np.zeros(len(rows) + 1, dtype=np.int64)
-    if rows.shape[1] == 8:
-        per = _lib.ADAMW_ITEM
-    else:
-        per = np.where(rows[:, 3] & 0xFFFFFFFF == _lib.DTYPE_F32, _lib.GRAD_ITEM_BYTES // 4, _lib.GRAD_ITEM_BYTES // 2)
-    np.cumsum(-(-rows[:, 2] // per), out=starts[1:])
+    n = rows[:, 2]
+    per, phase = _cuts(rows)
+    np.cumsum(np.where(n > 0, -(-(n + phase) // per), 0), out=starts[1:])
     host = torch.from_numpy(np.concatenate([rows.reshape(-1), starts]))
     if wait:
         table = host.to(device)
@@ -397,7 +405,7 @@ def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
 def _total_norm(tensors, device, norm: int, what: str) -> torch.Tensor:
     dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
     total = torch.empty((), dtype=torch.float32, device=device)
-    ws = _workspace(sum(_pieces(t) for t in dense), device)
+    ws = _workspace(sum(_most_pieces(t) for t in dense), device)
     _call(dense, device, "wq_grad_norm_few", "wq_grad_norm_items", what, (norm, 1.0, ws.data_ptr(), total.data_ptr()),
           lambda items, starts, n_items, n: (items, n_items, 4, starts, n, norm, 1.0, None, ws.data_ptr(), total.data_ptr(), None))
     return total
@@ -430,7 +438,8 @@ def _clip(grads, max_norm: float, norm: int, total_norm, what: str) -> torch.Ten
     work = dense + [c for _, c in copies]
     if total_norm is None:
         total = torch.empty((), dtype=torch.float32, device=device)
-        ws, given = _workspace(sum(_pieces(g) for g in work), device).data_ptr(), None
+        workspace = _workspace(sum(_most_pieces(g) for g in work), device)      # kept until the launches are out
+        ws, given = workspace.data_ptr(), None
     else:
         total = total_norm.detach().to(device=device, dtype=torch.float32)
         ws, given = None, total.data_ptr()

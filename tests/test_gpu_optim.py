@@ -273,6 +273,21 @@ def test_clip_takes_any_strides_and_refuses_shared_memory(cuda):
         slime_amd.clip_grad_norm_([p[0], p[0]], 5.0)
 
 
+@pytest.mark.parametrize("n", [3, 70])
+def test_clip_keeps_its_workspace_until_the_launch(cuda, monkeypatch, n):
+    import weakref
+
+    from slime_amd import optim
+
+    refs, workspace, call = [], optim._workspace, optim._call
+    monkeypatch.setattr(optim, "_workspace", lambda *a: refs.append(weakref.ref(t := workspace(*a))) or t)
+    monkeypatch.setattr(optim, "_call", lambda *a: call(*a) if refs[-1]() is not None else pytest.fail("the workspace is gone"))
+    ps = [torch.nn.Parameter(torch.zeros(50, device=cuda)) for _ in range(n)]
+    for p in ps:
+        p.grad = torch.ones(50, device=cuda)
+    assert abs(slime_amd.clip_grad_norm_(ps, 1.0).item() - math.sqrt(50 * n)) < 1e-4 and len(refs) == 1
+
+
 def test_clip_matches_torch(cuda):
     ps = [torch.nn.Parameter(torch.randn(s, device=cuda)) for s in ((64, 64), (100,), (3, 5, 7))]
     qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
@@ -530,6 +545,36 @@ def test_a_training_step_as_it_is_used(cuda):
             qe, se = slime_amd.blockwise_cast_to_fp8_triton(w.detach(), (128, 128))
             assert torch.equal(q.view(torch.uint8), qe.view(torch.uint8)) and torch.equal(sc, se)
             assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(sc, sc2)
+
+
+def test_item_tables_are_exact(cuda):
+    """Every row of a table of half a million pieces, from tensors of mixed types and starts (a per-lane 64-bit shift went wrong in
+    one wavefront of a hundred here)."""
+    import numpy as np
+
+    from slime_amd import optim
+
+    rng = np.random.default_rng(1)
+    base, rows = 0x7F0000000000, []
+    for i in range(400):
+        g, o = int(rng.integers(0, 3)), int(rng.integers(0, 3))
+        rows.append([base + 64 * i * 4, base + (1 << 40) + 2 * 64 * i + 4 * i, int(rng.integers(1, 20_000_000)) if i else (1 << 31) + 12345, g | o << 32])
+    for words in (4, 8):
+        if words == 8:
+            rows = [r + [base + (2 << 40) + 4 * i, base + (3 << 40), base + (4 << 40), i] for i, r in enumerate(rows)]
+        table = np.array(rows, dtype=np.int64)
+        items, starts, n = optim._item_table(table, cuda, "test", wait=True)
+        got, starts = items.cpu().numpy(), starts.cpu().numpy()
+        owner = np.repeat(np.arange(len(rows)), np.diff(starts))
+        per, phase = (np.broadcast_to(x, len(rows))[owner] for x in optim._cuts(table))
+        piece, src = np.arange(n) - starts[owner], table[owner]
+        at = np.where(piece > 0, piece * per - phase, 0)
+        g, o = (np.where(d == 1, 4, 2) for d in (src[:, 3] & 0xFFFFFFFF, src[:, 3] >> 32))
+        assert n > 300_000 and np.array_equal(got[:, 0], src[:, 0] + at * g) and np.array_equal(got[:, 1], src[:, 1] + at * o)
+        assert np.array_equal(got[:, 2], np.minimum((piece + 1) * per - phase, src[:, 2]) - at) and np.array_equal(got[:, 3], src[:, 3])
+        assert (np.add.reduceat(got[:, 2], starts[:-1]) == table[:, 2]).all()
+        for w in range(4, words):
+            assert np.array_equal(got[:, w], src[:, w] + (at * 4 if w < 7 else 0))
 
 
 def test_a_list_of_more_than_four_gigabytes(cuda):

@@ -256,3 +256,50 @@ def test_packed_floats_reach_the_descriptor():
     """lr_scale and weight_decay travel as the two halves of one 8-byte word, lr_scale first, as wq_adamw_desc has them."""
     word = np.array([[1.5, 0.25]], dtype=np.float32).view(np.int64)
     assert [ctypes.c_float.from_buffer_copy(word.tobytes()[i:i + 4]).value for i in (0, 4)] == [1.5, 0.25]
+
+
+def test_pieces_end_at_lines():
+    """The host's count of pieces is that of cutting at 128-byte lines of the stream that sets the pace."""
+    B, F = _lib.DTYPE_BF16, _lib.DTYPE_F32
+    rows = np.array([[128 + 2, 0, 5, B], [256, 256, 8192, B | B << 32], [256 + 2, 256 + 2, 8192, B | B << 32], [256, 512 + 4, 8192, B | F << 32],
+                     [256 + 4, 512, 4096, F | B << 32], [256, 512, 0, F | F << 32]], dtype=np.int64)
+    per, phase = optim._cuts(rows)
+    assert per.tolist() == [8192, 8192, 8192, 8192, 4096, 4096] and phase.tolist() == [1, 0, 1, 1, 1, 0]
+    adam = np.array([[64, 0, 9, F, 1024 + 124, 0, 0, 0]], dtype=np.int64)
+    per, phase = optim._cuts(adam)
+    assert per == _lib.ADAMW_ITEM and phase.tolist() == [31]
+    for ptr in range(0, 128, 4):
+        for n in (0, 1, 100, 4095, 4096, 4097, 12288):
+            t = torch.zeros(n)
+            count = 0 if n == 0 else -(-(n + ptr // 4) // 4096)
+            assert count <= optim._most_pieces(t)
+
+
+def test_no_64_bit_shift_by_a_vector_register(tmp_path):
+    """A 64-bit vector shift whose amount is in the last VGPR of a kernel goes wrong now and then on gfx950 (rows of an item
+    table came out unshifted), and the register allocator decides which kernel that hits: no kernel has such a shift by a
+    VGPR.  Compiles every kernel source with the library's own flags, as the test of flat instructions does."""
+    import concurrent.futures
+    import glob
+    import os
+    import re
+    import shutil
+    import subprocess
+
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "slime_amd", "csrc")
+    flags = re.search(r"^HIPFLAGS \?= (.*?)\n(?!\s)", open(os.path.join(csrc, "Makefile")).read(), re.S | re.M).group(1)
+    flags = flags.replace("\\\n", " ").replace("$(ARCH)", "gfx950").split()
+
+    def shifts(src):
+        out = tmp_path / (os.path.basename(src) + ".s")
+        subprocess.check_call([hipcc, *flags, "-S", "--cuda-device-only", "-o", str(out), src], stderr=subprocess.DEVNULL)
+        text = out.read_text()
+        assert "s_endpgm" in text or "wq_api" in src
+        return src, re.findall(r"v_(?:lshlrev_b64|lshrrev_b64|ashrrev_i64)\S* +\S+ +v\d+,.*", text)
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=4) as pool:
+        for src, found in pool.map(shifts, sorted(glob.glob(os.path.join(csrc, "*.hip")))):
+            assert not found, (os.path.basename(src), found)
