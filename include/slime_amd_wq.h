@@ -476,8 +476,9 @@ int wq_xxh3_128_grouped(const wq_xxh3_desc *descs, const int64_t *item_start, in
  *
  * Gradients are bf16, fp16 or fp32 (any alignment that their elements have), every tensor a flat run of n elements.  The
  * launches read one descriptor per piece - WQ_GRAD_ITEM_BYTES of a gradient, WQ_ADAMW_ITEM elements of a parameter - made from
- * per-tensor descriptors on the device by wq_grad_make_items; the *_few forms take up to WQ_GRAD_FEW_MAX per-tensor
- * descriptors from the HOST instead (read before the call returns).  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
+ * per-tensor descriptors on the device by wq_grad_make_items.  The *_list forms take HOST arrays of the tensors' addresses,
+ * element counts and types instead (read before the call returns) and pass them on in the kernel arguments,
+ * WQ_GRAD_LIST_LAUNCH tensors a launch: no table to build, upload or keep, any number of tensors.  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
  * call and neither overflow nor lose small gradients (fp32 squares exactly).
  *
  * grad_scale (an inverse loss scale, 1 / number of tokens ...) multiplies every gradient; if grad_scale_dev is not NULL the
@@ -486,7 +487,7 @@ int wq_xxh3_128_grouped(const wq_xxh3_desc *descs, const int64_t *item_start, in
  * infinite max_norm), as torch.nn.utils.clip_grads_with_norm_ has it. */
 #define WQ_GRAD_ITEM_BYTES 16384
 #define WQ_ADAMW_ITEM 8192
-#define WQ_GRAD_FEW_MAX 64
+#define WQ_GRAD_LIST_LAUNCH 176
 enum { WQ_NORM_2 = 0, WQ_NORM_INF = 1 };
 
 typedef struct wq_grad_desc {
@@ -528,8 +529,10 @@ int64_t wq_grad_workspace_bytes(int64_t n_items);
  * not read without `each`).  `words` as in wq_grad_make_items. */
 int wq_grad_norm_items(const void *items, int64_t n_items, int words, const int64_t *item_start, int n_desc, int norm,
                        float grad_scale, const float *grad_scale_dev, void *workspace, float *total, float *each, void *stream);
-int wq_grad_norm_few(const wq_grad_desc *descs, int n_desc, int norm, float grad_scale, void *workspace, float *total,
-                     void *stream);
+/* Workspace of the list forms (n_tensors >= 0; the arguments are those of the call); 0 for arguments that the call rejects. */
+int64_t wq_grad_list_workspace_bytes(const void *const *g, const int64_t *n, const int32_t *dtype, int n_tensors);
+int wq_grad_norm_list(const void *const *g, const int64_t *n, const int32_t *dtype, int n_tensors, int norm, float grad_scale,
+                      void *workspace, float *total, void *stream);
 
 /* out = round(g * coefficient).  With total_given NULL the norm is computed first and written to `total`; otherwise
  * total_given[0] is taken for it (a norm that was reduced over ranks) and workspace and total are not used.  Where a
@@ -537,8 +540,9 @@ int wq_grad_norm_few(const wq_grad_desc *descs, int n_desc, int norm, float grad
  * descriptors must not overlap each other or other descriptors' gradients. */
 int wq_grad_clip_items(const wq_grad_desc *items, int64_t n_items, int norm, float max_norm, float grad_scale,
                        const float *grad_scale_dev, const float *total_given, void *workspace, float *total, void *stream);
-int wq_grad_clip_few(const wq_grad_desc *descs, int n_desc, int norm, float max_norm, float grad_scale,
-                     const float *total_given, void *workspace, float *total, void *stream);
+/* in place */
+int wq_grad_clip_list(void *const *g, const int64_t *n, const int32_t *dtype, int n_tensors, int norm, float max_norm,
+                      float grad_scale, const float *total_given, void *workspace, float *total, void *stream);
 
 /* One AdamW step (decoupled weight decay), all arithmetic in fp32 from fp32 state, t = step + 1, g' = coefficient * g:
  *   p1 = p - lr * lr_scale * weight_decay * p;  m = b1 * m + (1 - b1) * g';  v = b2 * v + (1 - b2) * g'^2

@@ -28,7 +28,7 @@ INT4_DEQ_WORDS_PER_ITEM = 512
 BUCKET_COPY_MARK, BUCKET_COPY_BYTES = -1, 32768
 FP8_FEW_MAX = 4
 NORM_2, NORM_INF = 0, 1
-GRAD_ITEM_BYTES, ADAMW_ITEM, GRAD_FEW_MAX = 16384, 8192, 64
+GRAD_ITEM_BYTES, ADAMW_ITEM = 16384, 8192
 
 _i64, _int, _vp, _u32, _u64 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
 _f32, _f64 = ctypes.c_float, ctypes.c_double
@@ -86,9 +86,10 @@ SIGNATURES = {
     "wq_grad_make_items": [_vp, _vp, _int, _i64, _int, _vp, _vp],
     "wq_grad_workspace_bytes": [_i64],
     "wq_grad_norm_items": [_vp, _i64, _int, _vp, _int, _int, _f32, _vp, _vp, _vp, _vp, _vp],
-    "wq_grad_norm_few": [_vp, _int, _int, _f32, _vp, _vp, _vp],
+    "wq_grad_list_workspace_bytes": [_vp, _vp, _vp, _int],
+    "wq_grad_norm_list": [_vp, _vp, _vp, _int, _int, _f32, _vp, _vp, _vp],
     "wq_grad_clip_items": [_vp, _i64, _int, _f32, _f32, _vp, _vp, _vp, _vp, _vp],
-    "wq_grad_clip_few": [_vp, _int, _int, _f32, _f32, _vp, _vp, _vp, _vp],
+    "wq_grad_clip_list": [_vp, _vp, _vp, _int, _int, _f32, _f32, _vp, _vp, _vp, _vp],
     "wq_adamw_items": [_vp, _i64, ctypes.POINTER(AdamWHyper), _vp, _vp],
     "wq_delta_xor_xxh3": [_vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp],
 }
@@ -137,6 +138,14 @@ def check(rc: int, what: str) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """``stream_ptr`` of the device of this index without the Stream object that torch.cuda.current_stream makes (2 us)."""
+    return _current_raw_stream(index) if _current_raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

@@ -23,8 +23,10 @@ struct AdamControl {       // at the start of the workspace, written anew by eve
     float step_size;       // lr / (1 - b1^t)
     float inv_sqrt_bc2;    // 1 / sqrt(1 - b2^t)
     int32_t skip;
+    int32_t unused[3];
 };
-static_assert(sizeof(AdamControl) <= kGradControlBytes, "workspace layout");
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+static_assert(sizeof(AdamControl) == sizeof(u32x8) && sizeof(AdamControl) <= kGradControlBytes, "workspace layout");
 
 struct AdamBeginArgs {
     const char* partials;
@@ -142,15 +144,17 @@ __device__ __forceinline__ void adam_part_from(const AdamPart& d, const AdamCons
     else adam_part<G, WQ_DTYPE_F16>(d, k, s);
 }
 
-__global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc* items, const int64_t n_parts, const AdamConsts k,
+__global__ __launch_bounds__(kGradThreads) void adamw_kernel(const wq_adamw_desc* items, const int64_t n_parts, AdamConsts k,
                                                             const AdamControl* control)
 {
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-    if (slot >= n_parts) return;  // uniform per workgroup
-    const AdamControl c = *control;
-    if (c.skip) return;
-    const int64_t part = xcd_chunked_item(slot, n_parts, kAdamPartsPerXcdRun);
-    const wq_adamw_desc d = items[part / kAdamParts];
+    const int64_t part = item_of_slot(slot, n_parts, kAdamPartsPerXcdRun);
+    i64x8 w = *(const WQ_CONST i64x8*)((const int64_t*)items + part / kAdamParts * 8);
+    u32x8 cw = *(const WQ_CONST u32x8*)control;
+    asm volatile("" : "+s"(w), "+s"(cw), "+s"(k.beta1), "+s"(k.one_minus_beta1), "+s"(k.beta2), "+s"(k.one_minus_beta2), "+s"(k.eps));
+    const AdamControl c = __builtin_bit_cast(AdamControl, cw);
+    if (slot >= n_parts || c.skip) return;  // uniform per workgroup
+    const wq_adamw_desc d = __builtin_bit_cast(wq_adamw_desc, w);
     const Run r = run_of(part % kAdamParts, d.n, kAdamPart, phase_of(d.p, 4));
     if (r.n <= 0) return;
     const int at = (int)r.at;

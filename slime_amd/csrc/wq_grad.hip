@@ -17,7 +17,7 @@ constexpr int kLoads = 4;
 constexpr int kNormPiecesPerXcdRun = 32;
 constexpr unsigned kNormOccupancyPadBytes = 27000;   // 6 workgroups per CU
 constexpr int kScalePiecesPerXcdRun = 32;
-constexpr unsigned kScaleOccupancyPadBytes = 54000;  // 3
+constexpr unsigned kScaleOccupancyPadBytes = 40960;  // 4
 
 // ---- norm of a piece ------------------------------------------------------------------------------------------------
 template <int NORM, int D>
@@ -34,7 +34,9 @@ __device__ __forceinline__ void add_vec(typename NormAcc<NORM>::T& a, u32x4 v)
         }
     }
 }
-template <int NORM, int D>
+template <bool KEEP>
+__device__ __forceinline__ u32x4 load_grad(const char* p) { return KEEP ? ldg16(p) : ldg16_nt(p); }
+template <int NORM, int D, bool KEEP>
 __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece& p)
 {
     constexpr int kVec = 16 / dtype_bytes(D), kBatch = kLoads * kGradThreads;
@@ -45,10 +47,10 @@ __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece&
         u32x4 v[kLoads];
         if (b + kBatch <= whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(g + (size_t)(b + i * kGradThreads + t) * 16);
+            for (int i = 0; i < kLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)(b + i * kGradThreads + t) * 16);
         } else {  // lanes past the end load the last vector and count it as zeros
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = ldg16_nt(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
+            for (int i = 0; i < kLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
                 if (b + i * kGradThreads + t >= whole) v[i] = (u32x4){0u, 0u, 0u, 0u};
@@ -62,19 +64,20 @@ __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece&
     return a;
 }
 
-template <int NORM, typename Source>
+template <int NORM, bool KEEP, typename Source>
 __global__ __launch_bounds__(kGradThreads) void grad_norm_partials_kernel(const Source src, const int64_t n_items, char* partials)
 {
     typedef typename NormAcc<NORM>::T T;
     __shared__ T lds[kGradThreads / 64];
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    const int64_t item = item_of_slot(slot, n_items, kNormPiecesPerXcdRun);
+    GradPiece p = src.piece(item);
+    asm volatile("" : "+s"(p.g), "+s"(p.n), "+s"(p.g_dtype));
     if (slot >= n_items) return;  // uniform per workgroup
-    const int64_t item = xcd_chunked_item(slot, n_items, kNormPiecesPerXcdRun);
-    const GradPiece p = src.piece(item);
     T a;
-    if (p.g_dtype == WQ_DTYPE_BF16) a = piece_norm<NORM, WQ_DTYPE_BF16>(p);
-    else if (p.g_dtype == WQ_DTYPE_F16) a = piece_norm<NORM, WQ_DTYPE_F16>(p);
-    else a = piece_norm<NORM, WQ_DTYPE_F32>(p);
+    if (p.g_dtype == WQ_DTYPE_BF16) a = piece_norm<NORM, WQ_DTYPE_BF16, KEEP>(p);
+    else if (p.g_dtype == WQ_DTYPE_F16) a = piece_norm<NORM, WQ_DTYPE_F16, KEEP>(p);
+    else a = piece_norm<NORM, WQ_DTYPE_F32, KEEP>(p);
     a = block_fold<NORM, kGradThreads / 64>(a, lds);
     if (threadIdx.x == 0) stg<T>(partials + item * 8, a);
 }
@@ -90,13 +93,13 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_fold_kernel(const char
     if (threadIdx.x == 0) stg<T>(sums + (int64_t)blockIdx.x * 8, a);
 }
 
-template <int NORM>
-__global__ __launch_bounds__(1024) void grad_norm_total_kernel(const char* partials, const int64_t n, const float scale,
-                                                              const float* scale_dev, float* total)
+template <int NORM, int THREADS>
+__global__ __launch_bounds__(THREADS) void grad_norm_total_kernel(const char* partials, const int64_t n, const float scale,
+                                                                 const float* scale_dev, float* total)
 {
     typedef typename NormAcc<NORM>::T T;
-    __shared__ T lds[16];
-    const T a = fold_partials<NORM, 1024>(partials, n, lds);
+    __shared__ T lds[THREADS / 64];
+    const T a = fold_partials<NORM, THREADS>(partials, n, lds);
     if (threadIdx.x == 0) stg<float>(total, NormAcc<NORM>::finish(a, effective_scale(scale, scale_dev)));
 }
 
@@ -182,16 +185,28 @@ __device__ __forceinline__ void piece_scale_from(const GradPiece& p, float c)
     else piece_scale<G, WQ_DTYPE_F32>(p, c);
 }
 
-template <typename Source>
-__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_items, const float* total,
-                                                                 const float max_norm, const float scale, const float* scale_dev)
+// NORM < 0: the norm is at `total`.  Otherwise every workgroup folds the list's partials for itself - kFoldByAll at most, a
+// microsecond - in the order in which the total's kernel would, and the first one writes the norm: a launch less where the
+// launches are most of the time (router and norm vectors of a layer: 3 -> 2).
+template <int NORM, typename Source>
+__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_items, float* total, float max_norm,
+                                                                 float scale, const float* scale_dev, const Partials partials)
 {
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-    if (slot >= n_items) return;  // uniform per workgroup
-    const float c = clip_coefficient(ldg<float>(total), max_norm, effective_scale(scale, scale_dev));
-    // last piece first: what the norm read last is what a cache still holds
-    const GradPiece p = src.piece(n_items - 1 - xcd_chunked_item(slot, n_items, kScalePiecesPerXcdRun));
-    if (c == 1.0f && p.out == p.g) return;
+    GradPiece p = src.piece(item_of_slot(slot, n_items, kScalePiecesPerXcdRun));
+    uint32_t norm_bits = NORM < 0 ? const_u32(total) : 0u, dev = 0u;
+    if (NORM < 0) dev = const_u32(scale_dev ? scale_dev : total);
+    else if (scale_dev) dev = const_u32(scale_dev);
+    asm volatile("" : "+s"(p.g), "+s"(p.out), "+s"(p.n), "+s"(p.g_dtype), "+s"(p.out_dtype), "+s"(norm_bits), "+s"(dev), "+s"(max_norm), "+s"(scale));
+    const float s = scale_dev ? scale * u2f(dev) : scale;
+    float norm = u2f(norm_bits);
+    if constexpr (NORM >= 0) {
+        __shared__ typename NormAcc<NORM>::T lds[kGradThreads / 64];
+        norm = NormAcc<NORM>::finish(fold_partials<NORM, kGradThreads>(partials.at, partials.n, lds), s);
+        if (slot == 0 && threadIdx.x == 0) stg<float>(total, norm);
+    }
+    const float c = clip_coefficient(norm, max_norm, s);
+    if (slot >= n_items || (c == 1.0f && p.out == p.g)) return;  // uniform per workgroup
     if (p.g_dtype == WQ_DTYPE_BF16) piece_scale_from<WQ_DTYPE_BF16>(p, c);
     else if (p.g_dtype == WQ_DTYPE_F16) piece_scale_from<WQ_DTYPE_F16>(p, c);
     else piece_scale_from<WQ_DTYPE_F32>(p, c);
@@ -234,68 +249,153 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
     }
 }
 
+// A norm whose gradients are read again right away (`again`) leaves them in the 256 MB Infinity Cache if they fit: plain
+// instead of non-temporal loads make the norm alone slower (202 MB of bf16: 35 -> 38 us) and norm and clip together faster
+// (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 87 -> 81 us); with 2.4 GB nothing is left to find (1060 -> 1087 us).
+constexpr int64_t kKeepPieces = (256 << 20) / WQ_GRAD_ITEM_BYTES;
+
 template <int NORM, typename Source>
-static Partials launch_partials(const Source& src, int64_t n_items, void* workspace, hipStream_t st)
+static void launch_pieces(const Source& src, int64_t n_items, bool keep, char* partials, hipStream_t st)
 {
-    char* partials = partials_of(workspace);
-    if (n_items) grad_norm_partials_kernel<NORM><<<grid_for_items(n_items), kGradThreads, kNormOccupancyPadBytes, st>>>(src, n_items, partials);
+    if (n_items == 0) return;
+    const dim3 g = grid_for_items(n_items);
+    if (keep) grad_norm_partials_kernel<NORM, true><<<g, kGradThreads, kNormOccupancyPadBytes, st>>>(src, n_items, partials);
+    else grad_norm_partials_kernel<NORM, false><<<g, kGradThreads, kNormOccupancyPadBytes, st>>>(src, n_items, partials);
+}
+template <int NORM>
+static Partials launch_fold(char* partials, int64_t n_items, hipStream_t st)
+{
     if (n_items <= kFoldDirect) return {partials, n_items};
     const int64_t groups = cdiv64(n_items, kFoldGroup);
     char* sums = partials + n_items * 8;
     grad_norm_fold_kernel<NORM><<<(unsigned)groups, kGradThreads, 0, st>>>(partials, n_items, sums);
     return {sums, groups};
 }
+constexpr int64_t kFoldByAll = 1024;
+template <int NORM>
+static void launch_total(char* partials, int64_t n_items, float scale, const float* scale_dev, float* total, hipStream_t st)
+{
+    const Partials p = launch_fold<NORM>(partials, n_items, st);
+    if (n_items <= kFoldByAll) grad_norm_total_kernel<NORM, kGradThreads><<<1, kGradThreads, 0, st>>>(p.at, p.n, scale, scale_dev, total);
+    else grad_norm_total_kernel<NORM, 1024><<<1, 1024, 0, st>>>(p.at, p.n, scale, scale_dev, total);
+}
+template <int NORM>
+static Partials launch_table_partials(const TableSource& src, int64_t n_items, bool again, void* workspace, hipStream_t st)
+{
+    launch_pieces<NORM>(src, n_items, again && n_items <= kKeepPieces, partials_of(workspace), st);
+    return launch_fold<NORM>(partials_of(workspace), n_items, st);
+}
 Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st)
 {
-    return norm == WQ_NORM_2 ? launch_partials<WQ_NORM_2>(src, n_items, workspace, st) : launch_partials<WQ_NORM_INF>(src, n_items, workspace, st);
+    return norm == WQ_NORM_2 ? launch_table_partials<WQ_NORM_2>(src, n_items, true, workspace, st)
+                             : launch_table_partials<WQ_NORM_INF>(src, n_items, true, workspace, st);
 }
-
+template <int NORM>
+static void launch_table_norm(const TableSource& src, int64_t n_items, bool again, float scale, const float* scale_dev, void* workspace,
+                              float* total, hipStream_t st)
+{
+    launch_pieces<NORM>(src, n_items, again && n_items <= kKeepPieces, partials_of(workspace), st);
+    launch_total<NORM>(partials_of(workspace), n_items, scale, scale_dev, total, st);
+}
 template <int NORM, typename Source>
-static void launch_norm_kind(const Source& src, int64_t n_items, float scale, const float* scale_dev, void* workspace, float* total,
-                             hipStream_t st)
+static void launch_scale(const Source& src, int64_t n_items, float* total, float max_norm, float scale, const float* scale_dev,
+                         Partials partials, hipStream_t st)
 {
-    const Partials p = launch_partials<NORM>(src, n_items, workspace, st);
-    grad_norm_total_kernel<NORM><<<1, 1024, 0, st>>>(p.at, p.n, scale, scale_dev, total);
-}
-template <typename Source>
-static void launch_norm(const Source& src, int64_t n_items, int norm, float scale, const float* scale_dev, void* workspace,
-                        float* total, hipStream_t st)
-{
-    if (norm == WQ_NORM_2) launch_norm_kind<WQ_NORM_2>(src, n_items, scale, scale_dev, workspace, total, st);
-    else launch_norm_kind<WQ_NORM_INF>(src, n_items, scale, scale_dev, workspace, total, st);
-}
-template <typename Source>
-static void launch_clip(const Source& src, int64_t n_items, int norm, float max_norm, float scale, const float* scale_dev,
-                        const float* given, void* workspace, float* total, hipStream_t st)
-{
-    if (!given) launch_norm(src, n_items, norm, scale, scale_dev, workspace, total, st);
     if (n_items == 0) return;
-    grad_scale_kernel<<<grid_for_items(n_items), kGradThreads, kScaleOccupancyPadBytes, st>>>(src, n_items, given ? given : total,
-                                                                                              max_norm, scale, scale_dev);
+    grad_scale_kernel<NORM><<<grid_for_items(n_items), kGradThreads, kScaleOccupancyPadBytes, st>>>(src, n_items, total, max_norm, scale,
+                                                                                                    scale_dev, partials);
+}
+template <int NORM>
+static void launch_table_clip(const TableSource& src, int64_t n_items, float max_norm, float scale, const float* scale_dev,
+                              void* workspace, float* total, hipStream_t st)
+{
+    if (n_items == 0 || n_items > kFoldByAll) {
+        launch_table_norm<NORM>(src, n_items, true, scale, scale_dev, workspace, total, st);
+        launch_scale<-1>(src, n_items, total, max_norm, scale, scale_dev, Partials{}, st);
+    } else {
+        launch_pieces<NORM>(src, n_items, true, partials_of(workspace), st);
+        launch_scale<NORM>(src, n_items, total, max_norm, scale, scale_dev, Partials{partials_of(workspace), n_items}, st);
+    }
 }
 
 static bool grad_dtype_ok(int d) { return d == WQ_DTYPE_BF16 || d == WQ_DTYPE_F16 || d == WQ_DTYPE_F32; }
 
-// per-tensor HOST descriptors -> kernel arguments; negative: an error
-static int64_t few_source(const wq_grad_desc* descs, int n_desc, bool with_out, FewSource* src)
+// ---- HOST lists -----------------------------------------------------------------------------------------------------------
+struct HostList {
+    const void* const* g;
+    const int64_t* n;
+    const int32_t* dtype;
+    int n_tensors;
+    int64_t pieces(int i) const { return pieces_of(n[i], grad_item(dtype[i]), phase_of(g[i], dtype_bytes(dtype[i]))); }
+};
+// number of pieces of the whole list; negative: an error.  Looks at everything before anything is launched.
+static int64_t check_list(const HostList& l)
 {
-    if (n_desc < 0 || n_desc > WQ_GRAD_FEW_MAX) return WQ_ERR_SHAPE;
-    if (n_desc && !descs) return WQ_ERR_NULL;
-    int64_t items = 0;
-    int k = 0;
-    for (int i = 0; i < n_desc; ++i) {
-        if (descs[i].n < 0) return WQ_ERR_SHAPE;
-        if (!grad_dtype_ok(descs[i].g_dtype) || (with_out && !grad_dtype_ok(descs[i].out_dtype))) return WQ_ERR_MODE;
-        if (descs[i].n == 0) continue;
-        if (!descs[i].g || (with_out && !descs[i].out)) return WQ_ERR_NULL;
-        src->d[k] = descs[i];
-        if (!with_out) src->d[k].out = nullptr;
-        src->start[k++] = items;
-        items += pieces_of(descs[i].n, grad_item(descs[i].g_dtype), grad_phase(src->d[k - 1]));
+    if (l.n_tensors < 0) return WQ_ERR_SHAPE;
+    if (l.n_tensors && (!l.g || !l.n || !l.dtype)) return WQ_ERR_NULL;
+    int64_t total = 0;
+    for (int i = 0; i < l.n_tensors; ++i) {
+        if (l.n[i] < 0) return WQ_ERR_SHAPE;
+        if (!grad_dtype_ok(l.dtype[i])) return WQ_ERR_MODE;
+        if (l.n[i] > ((int64_t)1 << 40)) return WQ_ERR_TOO_LARGE;
+        if (l.n[i] && !l.g[i]) return WQ_ERR_NULL;
+        if ((uintptr_t)l.g[i] % dtype_bytes(l.dtype[i])) return WQ_ERR_ALIGN;
+        total += l.pieces(i);
+        if (total > ((int64_t)1 << 31) - 1) return WQ_ERR_TOO_LARGE;
     }
-    src->start[k] = items;
-    src->n_desc = k;
-    return items;
+    return total;
+}
+// calls launch(source, pieces of it, pieces before it) for every WQ_GRAD_LIST_LAUNCH tensors that have elements
+template <typename Launch>
+static void for_each_launch(const HostList& l, Launch launch)
+{
+    ListSource src;
+    int k = 0;
+    int64_t items = 0, before = 0;
+    for (int i = 0; i < l.n_tensors; ++i) {
+        if (l.n[i] == 0) continue;
+        src.g[k] = (const char*)l.g[i];
+        src.n_dtype[k] = (uint64_t)l.n[i] | (uint64_t)l.dtype[i] << 56;
+        src.start[k++] = (int32_t)items;
+        items += l.pieces(i);
+        if (k == WQ_GRAD_LIST_LAUNCH) {
+            src.n_tensors = k;
+            launch(src, items, before);
+            before += items;
+            k = 0, items = 0;
+        }
+    }
+    src.n_tensors = k;
+    if (k) launch(src, items, before);
+}
+template <int NORM>
+static void launch_list_pieces(const HostList& l, bool keep, char* partials, hipStream_t st)
+{
+    for_each_launch(l, [&](const ListSource& src, int64_t items, int64_t before) { launch_pieces<NORM>(src, items, keep, partials + before * 8, st); });
+}
+template <int NORM>
+static void launch_list_norm(const HostList& l, int64_t pieces, float scale, void* workspace, float* total, hipStream_t st)
+{
+    launch_list_pieces<NORM>(l, false, partials_of(workspace), st);
+    launch_total<NORM>(partials_of(workspace), pieces, scale, nullptr, total, st);
+}
+static void launch_list_scale(const HostList& l, float* total, float max_norm, float scale, hipStream_t st)
+{
+    for_each_launch(l, [&](const ListSource& src, int64_t items, int64_t) { launch_scale<-1>(src, items, total, max_norm, scale, nullptr, Partials{}, st); });
+}
+template <int NORM>
+static void launch_list_clip(const HostList& l, int64_t pieces, float max_norm, float scale, void* workspace, float* total, hipStream_t st)
+{
+    char* partials = partials_of(workspace);
+    launch_list_pieces<NORM>(l, pieces <= kKeepPieces, partials, st);
+    if (pieces == 0 || pieces > kFoldByAll || l.n_tensors > WQ_GRAD_LIST_LAUNCH) {
+        launch_total<NORM>(partials, pieces, scale, nullptr, total, st);
+        launch_list_scale(l, total, max_norm, scale, st);
+    } else {
+        for_each_launch(l, [&](const ListSource& src, int64_t items, int64_t) {
+            launch_scale<NORM>(src, items, total, max_norm, scale, nullptr, Partials{partials, pieces}, st);
+        });
+    }
 }
 
 }  // namespace wq
@@ -325,7 +425,9 @@ WQ_EXPORT int wq_grad_norm_items(const void* items, int64_t n_items, int words, 
     if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
     if (!workspace || !total || (n_items && !items) || (each && n_desc && !item_start)) return WQ_ERR_NULL;
     hipStream_t st = (hipStream_t)stream;
-    launch_norm(TableSource{(const int64_t*)items, words}, n_items, norm, grad_scale, grad_scale_dev, workspace, total, st);
+    const TableSource src = {(const int64_t*)items, words};
+    if (norm == WQ_NORM_2) launch_table_norm<WQ_NORM_2>(src, n_items, false, grad_scale, grad_scale_dev, workspace, total, st);
+    else launch_table_norm<WQ_NORM_INF>(src, n_items, false, grad_scale, grad_scale_dev, workspace, total, st);
     if (each && n_desc) {
         const char* partials = partials_of(workspace);
         if (norm == WQ_NORM_2) grad_norm_each_kernel<WQ_NORM_2><<<n_desc, kGradThreads, 0, st>>>(partials, item_start, grad_scale, grad_scale_dev, each);
@@ -335,15 +437,22 @@ WQ_EXPORT int wq_grad_norm_items(const void* items, int64_t n_items, int words, 
     return WQ_OK;
 }
 
-WQ_EXPORT int wq_grad_norm_few(const wq_grad_desc* descs, int n_desc, int norm, float grad_scale, void* workspace, float* total,
-                               void* stream)
+WQ_EXPORT int64_t wq_grad_list_workspace_bytes(const void* const* g, const int64_t* n, const int32_t* dtype, int n_tensors)
+{
+    const int64_t pieces = check_list({g, n, dtype, n_tensors});
+    return pieces < 0 ? 0 : wq_grad_workspace_bytes(pieces);
+}
+
+WQ_EXPORT int wq_grad_norm_list(const void* const* g, const int64_t* n, const int32_t* dtype, int n_tensors, int norm, float grad_scale,
+                                void* workspace, float* total, void* stream)
 {
     if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
-    FewSource src;
-    const int64_t items = few_source(descs, n_desc, false, &src);
-    if (items < 0) return (int)items;
+    const HostList l = {g, n, dtype, n_tensors};
+    const int64_t pieces = check_list(l);
+    if (pieces < 0) return (int)pieces;
     if (!workspace || !total) return WQ_ERR_NULL;
-    launch_norm(src, items, norm, grad_scale, nullptr, workspace, total, (hipStream_t)stream);
+    if (norm == WQ_NORM_2) launch_list_norm<WQ_NORM_2>(l, pieces, grad_scale, workspace, total, (hipStream_t)stream);
+    else launch_list_norm<WQ_NORM_INF>(l, pieces, grad_scale, workspace, total, (hipStream_t)stream);
     WQ_LAUNCH_CHECK();
     return WQ_OK;
 }
@@ -355,22 +464,28 @@ WQ_EXPORT int wq_grad_clip_items(const wq_grad_desc* items, int64_t n_items, int
     if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
     if ((!total_given && (!workspace || !total)) || (n_items && !items)) return WQ_ERR_NULL;
     if (n_items == 0 && total_given) return WQ_OK;
-    launch_clip(TableSource{(const int64_t*)items, 4}, n_items, norm, max_norm, grad_scale, grad_scale_dev, total_given, workspace,
-                total, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    const TableSource src = {(const int64_t*)items, 4};
+    if (total_given) launch_scale<-1>(src, n_items, const_cast<float*>(total_given), max_norm, grad_scale, grad_scale_dev, Partials{}, st);
+    else if (norm == WQ_NORM_2) launch_table_clip<WQ_NORM_2>(src, n_items, max_norm, grad_scale, grad_scale_dev, workspace, total, st);
+    else launch_table_clip<WQ_NORM_INF>(src, n_items, max_norm, grad_scale, grad_scale_dev, workspace, total, st);
     WQ_LAUNCH_CHECK();
     return WQ_OK;
 }
 
-WQ_EXPORT int wq_grad_clip_few(const wq_grad_desc* descs, int n_desc, int norm, float max_norm, float grad_scale,
-                               const float* total_given, void* workspace, float* total, void* stream)
+WQ_EXPORT int wq_grad_clip_list(void* const* g, const int64_t* n, const int32_t* dtype, int n_tensors, int norm, float max_norm,
+                                float grad_scale, const float* total_given, void* workspace, float* total, void* stream)
 {
     if (norm != WQ_NORM_2 && norm != WQ_NORM_INF) return WQ_ERR_MODE;
-    FewSource src;
-    const int64_t items = few_source(descs, n_desc, true, &src);
-    if (items < 0) return (int)items;
+    const HostList l = {g, n, dtype, n_tensors};
+    const int64_t pieces = check_list(l);
+    if (pieces < 0) return (int)pieces;
     if (!total_given && (!workspace || !total)) return WQ_ERR_NULL;
-    if (items == 0 && total_given) return WQ_OK;
-    launch_clip(src, items, norm, max_norm, grad_scale, nullptr, total_given, workspace, total, (hipStream_t)stream);
+    if (pieces == 0 && total_given) return WQ_OK;
+    hipStream_t st = (hipStream_t)stream;
+    if (total_given) launch_list_scale(l, const_cast<float*>(total_given), max_norm, grad_scale, st);
+    else if (norm == WQ_NORM_2) launch_list_clip<WQ_NORM_2>(l, pieces, max_norm, grad_scale, workspace, total, st);
+    else launch_list_clip<WQ_NORM_INF>(l, pieces, max_norm, grad_scale, workspace, total, st);
     WQ_LAUNCH_CHECK();
     return WQ_OK;
 }

@@ -17,6 +17,7 @@ constexpr int kAdamItem = WQ_ADAMW_ITEM;
 // anywhere): gfx950's global accesses take any address, the type says so to the compiler.
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ u32x4 ldg16(const char* p) { return *(const WQ_GLOBAL u32x4_a2*)p; }
 __device__ __forceinline__ u32x4 ldg16_nt(const char* p) { return __builtin_nontemporal_load((const WQ_GLOBAL u32x4_a2*)p); }
 __device__ __forceinline__ u32x2 ldg8_nt(const char* p) { return __builtin_nontemporal_load((const WQ_GLOBAL u32x2_a2*)p); }
 
@@ -88,32 +89,52 @@ struct GradPiece {
     char* out;
     int n, g_dtype, out_dtype;
 };
+// A workgroup lives for a few microseconds, and scalar loads that wait for one another (arguments, then the row, then a
+// step's scalars ...) are a good part of it: everything a workgroup needs is addressed without a branch and loaded at once -
+// a slot behind the last piece reads the last one's row and leaves after that -, and one empty asm that takes all of it keeps
+// the compiler from moving a load behind the branches that follow.  WQ_CONST: memory that no one writes while the kernel runs
+// (scalar loads).
+#define WQ_CONST __attribute__((address_space(4)))
+typedef int64_t i64x4 __attribute__((ext_vector_type(4), aligned(8)));
+typedef int64_t i64x8 __attribute__((ext_vector_type(8), aligned(8)));
+__device__ __forceinline__ uint32_t const_u32(const void* p) { return *(const WQ_CONST uint32_t*)p; }
+// the slot's work item (see xcd_chunked_item), without a branch; total > 0
+__device__ __forceinline__ int64_t item_of_slot(int64_t slot, int64_t total, int C)
+{
+    slot = slot < total ? slot : total - 1;
+    const int64_t span = (int64_t)kXcds * C, from = slot / span * span;
+    const uint32_t r = (uint32_t)(slot - from);
+    const int64_t mixed = from + (int64_t)(r % kXcds * C + r / kXcds), whole = -(int64_t)(from + span <= total);
+    return (mixed & whole) | (slot & ~whole);
+}
+
 // A table with one descriptor per piece; `words` is 4 (wq_grad_desc) or 8 (wq_adamw_desc, which begins alike).
 struct TableSource {
     const int64_t* items;
     int words;
     __device__ __forceinline__ GradPiece piece(int64_t t) const
     {
-        const wq_grad_desc* d = (const wq_grad_desc*)(items + t * words);
-        return {(const char*)d->g, (char*)d->out, (int)d->n, d->g_dtype, d->out_dtype};
+        const i64x4 d = *(const WQ_CONST i64x4*)(items + t * words);
+        return {(const char*)d[0], (char*)d[1], (int)d[2], (int)(uint32_t)d[3], (int)((uint64_t)d[3] >> 32)};
     }
 };
-// Per-tensor descriptors in the kernel arguments.
-struct FewSource {
-    wq_grad_desc d[WQ_GRAD_FEW_MAX];
-    int64_t start[WQ_GRAD_FEW_MAX + 1];
-    int n_desc;
+// Tensors in the kernel arguments (3.5 of their 4 KiB).
+struct ListSource {
+    const char* g[WQ_GRAD_LIST_LAUNCH];
+    uint64_t n_dtype[WQ_GRAD_LIST_LAUNCH];     // elements, type in the top byte
+    int32_t start[WQ_GRAD_LIST_LAUNCH];
+    int32_t n_tensors;
     __device__ __forceinline__ GradPiece piece(int64_t t) const
     {
-        int lo = 0, hi = n_desc;
+        int lo = 0, hi = n_tensors;
         while (hi - lo > 1) {  // start[lo] <= t < start[hi]
             const int mid = (lo + hi) >> 1;
             if (start[mid] <= t) lo = mid; else hi = mid;
         }
-        const Run r = run_of(t - start[lo], d[lo].n, grad_item(d[lo].g_dtype), grad_phase(d[lo]));
-        // norms leave `out` NULL and do not look at it
-        return {(const char*)d[lo].g + r.at * dtype_bytes(d[lo].g_dtype), (char*)d[lo].out + r.at * dtype_bytes(d[lo].out_dtype),
-                r.n, d[lo].g_dtype, d[lo].out_dtype};
+        const int dtype = (int)(n_dtype[lo] >> 56), bytes = dtype_bytes(dtype);
+        const Run r = run_of(t - start[lo], (int64_t)(n_dtype[lo] & ~(255ull << 56)), grad_item(dtype), phase_of(g[lo], bytes));
+        const char* at = g[lo] + r.at * bytes;
+        return {at, (char*)at, r.n, dtype, dtype};
     }
 };
 
@@ -204,7 +225,7 @@ struct Partials {
     int64_t n;
 };
 
-// wq_grad.hip: one partial per piece, folded to at most kFoldDirect (or n_items / kFoldGroup) values for a last fold
+// wq_grad.hip: one partial per piece (of gradients that are read again right behind), folded to at most kFoldDirect (or n_items / kFoldGroup) values for a last fold
 Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st);
 
 }  // namespace wq

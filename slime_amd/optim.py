@@ -16,8 +16,9 @@ Norm of a model that is sharded over ranks: ``norm = plan.run(); total = norm.sq
 
 from __future__ import annotations
 
-import array
 import math
+from array import array
+from contextlib import nullcontext
 from typing import Iterable, Sequence
 
 import numpy as np
@@ -125,23 +126,20 @@ def _scale_args(scale, device, what: str):
 def _launch(device: torch.device, entry: str, what: str, *args) -> None:
     fn = getattr(_lib.load(), entry)
     if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _lib.stream_ptr(device))
+        rc = fn(*args, _lib.raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _lib.stream_ptr(device))
-    _lib.check(rc, what)
+            rc = fn(*args, _lib.raw_stream(device.index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _bump(tensors) -> None:
     """Tell autograd that a kernel wrote into these tensors, as torch's in-place operations do."""
-    tensors = [t for t in tensors if not t.is_inference()]
-    if tensors:
+    try:
         torch.autograd.graph.increment_version(tensors)
-
-
-def _most_pieces(t) -> int:
-    """At least the number of pieces of a gradient, wherever it starts."""
-    return t.numel() * t.element_size() // _lib.GRAD_ITEM_BYTES + 2
+    except RuntimeError:                    # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _workspace(n_items: int, device) -> torch.Tensor:
@@ -162,18 +160,14 @@ def _cuts(rows: np.ndarray):
     return _lib.GRAD_ITEM_BYTES // g, np.where((rows[:, 1] != 0) & (o >= g), rows[:, 1] % 128 // o, rows[:, 0] % 128 // g)
 
 
-def _item_table(rows: np.ndarray, device, what: str, wait: bool):
+def _item_table(rows: np.ndarray, device, what: str):
     """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
-    of the tensors in it).  Without ``wait`` the upload goes through pinned memory and the host goes on."""
+    of the tensors in it, number of items)."""
     starts = np.zeros(len(rows) + 1, dtype=np.int64)
     n = rows[:, 2]
     per, phase = _cuts(rows)
     np.cumsum(np.where(n > 0, -(-(n + phase) // per), 0), out=starts[1:])
-    host = torch.from_numpy(np.concatenate([rows.reshape(-1), starts]))
-    if wait:
-        table = host.to(device)
-    else:
-        table = host.pin_memory().to(device, non_blocking=True)
+    table = torch.from_numpy(np.concatenate([rows.reshape(-1), starts])).to(device)
     n_items, words = int(starts[-1]), rows.shape[1]
     items = torch.empty((max(n_items, 1), words), dtype=torch.int64, device=device)
     start_t = table[rows.size:]
@@ -188,7 +182,7 @@ class _Plan:
     def _build(self, rows, device, what: str) -> None:
         self.device, self._what = device, what
         with torch.cuda.device(device):
-            self._items, self._starts, self._n_items = _item_table(np.array(rows, dtype=np.int64), device, what, wait=True)
+            self._items, self._starts, self._n_items = _item_table(np.array(rows, dtype=np.int64), device, what)
             self._workspace = _workspace(self._n_items, device)
             self.total_norm = torch.zeros((), dtype=torch.float32, device=device)
             self._stream = torch.cuda.current_stream(device)
@@ -198,8 +192,8 @@ class _Plan:
         self._stream.synchronize()      # a run on another stream finds the tables ready
 
     def _run(self, entry: str, *args) -> None:
-        stream = torch.cuda.current_stream(self.device)
-        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+        if _lib.raw_stream(self.device.index) != self._stream.cuda_stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.device)
             for t in self._owned:       # the allocator must not hand them out while this stream may still use them
                 t.record_stream(stream)
         _launch(self.device, entry, self._what, *args)
@@ -351,15 +345,17 @@ class AdamWPlan(_Plan):
         self.skip_nonfinite = bool(skip_nonfinite)
         self.step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._owned.append(self.step)
+        self._hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, 0.0, None, None, None, self.total_norm.data_ptr(),
+                                      self.step.data_ptr(), 1.0, -1.0, self._norm, self.skip_nonfinite)
         self._built()
 
     def run(self, lr, max_norm: float | None = None, grad_scale=1.0, total_norm: torch.Tensor | None = None):
         max_norm = -1.0 if max_norm is None else _check_max_norm(max_norm, "AdamWPlan")
-        scale, scale_dev = _scale_args(grad_scale, self.device, "AdamWPlan: grad_scale")
-        lr, lr_dev = _scale_args(lr, self.device, "AdamWPlan: lr")
-        hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, lr, lr_dev, scale_dev, self._given(total_norm),
-                                self.total_norm.data_ptr(), self.step.data_ptr(), scale, max_norm, self._norm, self.skip_nonfinite)
-        self._run("wq_adamw_items", self._items.data_ptr(), self._n_items, hyper, self._workspace.data_ptr())
+        h = self._hyper
+        h.lr, h.lr_dev = _scale_args(lr, self.device, "AdamWPlan: lr")
+        h.grad_scale, h.grad_scale_dev = _scale_args(grad_scale, self.device, "AdamWPlan: grad_scale")
+        h.total_given, h.max_norm = self._given(total_norm), max_norm
+        self._run("wq_adamw_items", self._items.data_ptr(), self._n_items, h, self._workspace.data_ptr())
         _bump(self._written)
         if max_norm < 0.0 and not self.skip_nonfinite:
             return None
@@ -371,28 +367,73 @@ class AdamWPlan(_Plan):
 def _grads_of(parameters) -> list:
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    return [p.grad for p in parameters if p.grad is not None]
+    return [g for p in parameters if (g := p.grad) is not None]
 
 
-def _checked(tensors, what: str):
-    for t in tensors:
-        _check_tensor(t, what)
-    return _one_device(tensors, what)
+_data_ptr, _numel, _is_contiguous, _get_device = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device"))
+_dtype = torch.Tensor.dtype.__get__
+_PLAIN_TYPES = {torch.Tensor, torch.nn.Parameter}
 
 
-def _call(tensors, device, few: str, many: str, what: str, few_args, many_args) -> None:
-    """The launch over ``tensors``: descriptors in the kernel arguments, or a table made for this call."""
-    n = len(tensors)
-    rows = [_grad_row(t) for t in tensors]
-    if n <= _lib.GRAD_FEW_MAX:
-        host = array.array("q", [x for row in rows for x in row])
-        _launch(device, few, what, host.buffer_info()[0], n, *few_args)
-        return
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what}: a call over more than {_lib.GRAD_FEW_MAX} tensors cannot be captured; use a plan")
-    with torch.cuda.device(device):
-        items, starts, n_items = _item_table(np.array(rows, dtype=np.int64), device, what, wait=False)
-    _launch(device, many, what, *many_args(items.data_ptr(), starts.data_ptr(), n_items, n))
+class _List:
+    """Tensors as the list entry points take them: host arrays of addresses, element counts and types.  The common case -
+    contiguous tensors of one GPU - is found out by passes that stay in C (0.2 us a tensor); anything else is looked at
+    one by one, for the message or for the copies that other strides need."""
+
+    def __init__(self, tensors, what: str, written: bool):
+        self.copies = []
+        selectors = None
+        if set(map(type, tensors)) <= _PLAIN_TYPES:
+            try:
+                index = set(map(_get_device, tensors))
+                if len(index) == 1 and all(map(_is_contiguous, tensors)):
+                    self.index = index.pop()
+                    selectors = list(map(_DTYPES.get, map(_dtype, tensors)))
+            except RuntimeError:            # a layout without strides
+                pass
+        if selectors is None or None in selectors or self.index < 0:
+            tensors, selectors = self._one_by_one(tensors, what, written)
+        self.tensors, self.device = tensors, torch.device("cuda", self.index)
+        self.ptr, self.n = array("q", map(_data_ptr, tensors)), array("q", map(_numel, tensors))
+        self.dtype = array("i", selectors)
+        if written:
+            self._refuse_overlaps(what)
+        self.args = (self.ptr.buffer_info()[0], self.n.buffer_info()[0], self.dtype.buffer_info()[0], len(tensors))
+
+    def _one_by_one(self, tensors, what: str, written: bool):
+        for t in tensors:
+            _check_tensor(t, what)
+        self.index = _one_device(tensors, what).index
+        dense = []
+        for t in tensors:
+            if _is_dense(t):
+                dense.append(t)
+                continue
+            if written:
+                _check_no_self_overlap(t, what)
+            copy = t.contiguous()
+            dense.append(copy)
+            self.copies.append((t, copy))
+        return dense, [_DTYPES[t.dtype] for t in dense]
+
+    def _refuse_overlaps(self, what: str) -> None:
+        if len(self.ptr) <= 16:             # the arrays below cost 8 us however short they are
+            spans = sorted((p, p + n * (4 if d == _lib.DTYPE_F32 else 2)) for p, n, d in zip(self.ptr, self.n, self.dtype) if n)
+            overlap = any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+        else:
+            at, n = np.frombuffer(self.ptr, np.int64), np.frombuffer(self.n, np.int64)
+            order = np.argsort(at[n > 0], kind="stable")
+            start = at[n > 0][order]
+            end = start + (n * np.where(np.frombuffer(self.dtype, np.int32) == _lib.DTYPE_F32, 4, 2))[n > 0][order]
+            overlap = (start[1:] < end[:-1]).any()
+        if overlap:
+            raise ValueError(f"{what}: gradients share memory (the same tensor twice?); they cannot be clipped in place")
+
+    def workspace(self) -> torch.Tensor:
+        """Kept by the caller until the launches are out; what comes after them on the stream may reuse it.  Large enough for
+        any list of these sizes: as many pieces as fp32 has, and two more per tensor for where it starts."""
+        pieces = sum(self.n) * 4 // _lib.GRAD_ITEM_BYTES + 2 * len(self.n)
+        return torch.empty(8 + pieces + pieces // 4096 + 1, dtype=torch.int64, device=self.device)
 
 
 def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
@@ -402,12 +443,10 @@ def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
                            "`error_if_nonfinite=False`")
 
 
-def _total_norm(tensors, device, norm: int, what: str) -> torch.Tensor:
-    dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
-    total = torch.empty((), dtype=torch.float32, device=device)
-    ws = _workspace(sum(_most_pieces(t) for t in dense), device)
-    _call(dense, device, "wq_grad_norm_few", "wq_grad_norm_items", what, (norm, 1.0, ws.data_ptr(), total.data_ptr()),
-          lambda items, starts, n_items, n: (items, n_items, 4, starts, n, norm, 1.0, None, ws.data_ptr(), total.data_ptr(), None))
+def _total_norm(tensors: _List, norm: int, what: str) -> torch.Tensor:
+    device = tensors.device
+    total, workspace = torch.empty((), dtype=torch.float32, device=device), tensors.workspace()
+    _launch(device, "wq_grad_norm_list", what, *tensors.args, norm, 1.0, workspace.data_ptr(), total.data_ptr())
     return total
 
 
@@ -419,39 +458,27 @@ def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: fl
     norm = _norm_selector(norm_type, "get_total_norm")
     if not tensors:
         return torch.tensor(0.0)
-    total = _total_norm(tensors, _checked(tensors, "get_total_norm"), norm, "get_total_norm")
+    total = _total_norm(_List(tensors, "get_total_norm", written=False), norm, "get_total_norm")
     if error_if_nonfinite:
         _refuse_nonfinite(total, norm_type)
     return total
 
 
-def _clip(grads, max_norm: float, norm: int, total_norm, what: str) -> torch.Tensor:
-    device = _checked(grads, what)
-    dense, copies = [], []
-    for g in grads:
-        if _is_dense(g):
-            dense.append(g)
-        else:
-            _check_no_self_overlap(g, what)
-            copies.append((g, g.contiguous()))
-    _refuse_overlaps(dense, (), what)
-    work = dense + [c for _, c in copies]
+def _clip(grads: _List, max_norm: float, norm: int, total_norm, what: str) -> torch.Tensor:
+    device = grads.device
     if total_norm is None:
-        total = torch.empty((), dtype=torch.float32, device=device)
-        workspace = _workspace(sum(_most_pieces(g) for g in work), device)      # kept until the launches are out
-        ws, given = workspace.data_ptr(), None
+        total, workspace = torch.empty((), dtype=torch.float32, device=device), grads.workspace()
+        _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, None, workspace.data_ptr(), total.data_ptr())
     else:
         total = total_norm.detach().to(device=device, dtype=torch.float32)
-        ws, given = None, total.data_ptr()
-    _call(work, device, "wq_grad_clip_few", "wq_grad_clip_items", what, (norm, max_norm, 1.0, given, ws, total.data_ptr()),
-          lambda items, _, n_items, n: (items, n_items, norm, max_norm, 1.0, None, given, ws, total.data_ptr()))
-    _bump(dense)
-    for g, c in copies:
-        g.copy_(c)
+        _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, total.data_ptr(), None, None)
+    _bump(grads.tensors)
+    with torch.no_grad() if grads.copies else nullcontext():
+        for t, copy in grads.copies:
+            t.copy_(copy)
     return total
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` for bf16 / fp16 / fp32 gradients on one GPU: scales the gradients in place by
@@ -461,14 +488,13 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     grads = _grads_of(parameters)
     if not grads:
         return torch.tensor(0.0)
-    total = None
+    grads, total = _List(grads, "clip_grad_norm_", written=True), None
     if error_if_nonfinite:
-        total = _total_norm(grads, _checked(grads, "clip_grad_norm_"), norm, "clip_grad_norm_")
+        total = _total_norm(grads, norm, "clip_grad_norm_")
         _refuse_nonfinite(total, norm_type)
     return _clip(grads, max_norm, norm, total, "clip_grad_norm_")
 
 
-@torch.no_grad()
 def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor,
                           foreach: bool | None = None) -> None:
     """``torch.nn.utils.clip_grads_with_norm_``: the clip alone, by a norm that the caller has (reduced over ranks, say)."""
@@ -477,4 +503,5 @@ def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max
         raise TypeError("clip_grads_with_norm_: total_norm must be a tensor of one value")
     grads = _grads_of(parameters)
     if grads:
-        _clip(grads, max_norm, _lib.NORM_2, total_norm, "clip_grads_with_norm_")
+        what = "clip_grads_with_norm_"
+        _clip(_List(grads, what, written=True), max_norm, _lib.NORM_2, total_norm, what)

@@ -36,36 +36,47 @@ def test_entry_points_reject_bad_arguments():
     assert lib.wq_grad_norm_items(P, 1, 4, None, 0, 0, 1.0, None, None, P, None, None) == N_
     assert lib.wq_grad_norm_items(P, 1, 4, None, 0, 0, 1.0, None, P, None, None, None) == N_
     assert lib.wq_grad_norm_items(P, 1, 4, None, 2, 0, 1.0, None, P, P, P, None) == N_          # `each` without the starts
-    assert lib.wq_grad_norm_few(None, _lib.GRAD_FEW_MAX + 1, 0, 1.0, P, P, None) == S
-    assert lib.wq_grad_norm_few(None, -1, 0, 1.0, P, P, None) == S
-    assert lib.wq_grad_norm_few(None, 2, 0, 1.0, P, P, None) == N_
-    assert lib.wq_grad_norm_few(None, 0, 7, 1.0, P, P, None) == M_
-    assert lib.wq_grad_norm_few(None, 0, 0, 1.0, None, P, None) == N_
     assert lib.wq_grad_clip_items(None, 2, 0, 1.0, 1.0, None, None, P, P, None) == N_
     assert lib.wq_grad_clip_items(P, 2, 0, 1.0, 1.0, None, None, None, P, None) == N_
     assert lib.wq_grad_clip_items(P, -2, 0, 1.0, 1.0, None, P, None, None, None) == S
     assert lib.wq_grad_clip_items(P, 2, 5, 1.0, 1.0, None, P, None, None, None) == M_
     assert lib.wq_grad_clip_items(None, 0, 0, 1.0, 1.0, None, P, None, None, None) == 0         # nothing to do
-    assert lib.wq_grad_clip_few(None, 3, 0, 1.0, 1.0, P, None, None, None) == N_
-    assert lib.wq_grad_clip_few(None, 0, 0, 1.0, 1.0, P, None, None, None) == 0
 
 
-def _few(**change):
-    d = {"g": 64, "out": 64, "n": 5, "g_dtype": _lib.DTYPE_F32, "out_dtype": _lib.DTYPE_F32}
-    d.update(change)
-    return (ctypes.c_int64 * 4)(d["g"], d["out"], d["n"], d["g_dtype"] | d["out_dtype"] << 32)
+class _Host:
+    """A host list; pointers are never followed."""
+
+    def __init__(self, g=64, n=5, dtype=_lib.DTYPE_F32, count=1):
+        self.keep = [(ctypes.c_int64 * 2)(64, g), (ctypes.c_int64 * 2)(3, n), (ctypes.c_int32 * 2)(_lib.DTYPE_BF16, dtype)]
+        self.args = [*self.keep, 2]
+
+    def norm(self, ws=None, total=None, kind=0):
+        return _lib.load().wq_grad_norm_list(*self.args, kind, 1.0, ws, total, None)
+
+    def clip(self, given=None, ws=None, total=None, kind=0):
+        return _lib.load().wq_grad_clip_list(*self.args, kind, 1.0, 1.0, given, ws, total, None)
+
+    def bytes(self):
+        return _lib.load().wq_grad_list_workspace_bytes(*self.args)
 
 
-def test_host_descriptors_are_checked():
+def test_host_lists_are_checked():
     lib = _lib.load()
-    norm = lambda d: lib.wq_grad_norm_few(d, 1, 0, 1.0, None, None, None)      # noqa: E731  stops at the missing workspace
-    clip = lambda d: lib.wq_grad_clip_few(d, 1, 0, 1.0, 1.0, None, None, None, None)  # noqa: E731
-    assert norm(_few()) == clip(_few()) == N_
-    assert norm(_few(n=-1)) == clip(_few(n=-1)) == S
-    assert norm(_few(g_dtype=_lib.DTYPE_F64)) == clip(_few(g_dtype=9)) == M_
-    assert clip(_few(out_dtype=_lib.DTYPE_F64)) == M_
-    assert norm(_few(out_dtype=_lib.DTYPE_F64, out=0)) == N_                    # a norm looks at neither
-    assert clip(_few(out=0)) == N_ and norm(_few(g=0)) == N_
+    good = _Host()
+    assert good.norm() == good.clip() == good.norm(ws=P) == good.norm(total=P) == good.clip(total=P) == N_     # nowhere to put it
+    assert good.norm(kind=2) == good.clip(kind=-1) == M_
+    assert good.bytes() >= 64 + 2 * 8
+    for bad, code in ((_Host(n=-1), S), (_Host(dtype=_lib.DTYPE_F64), M_), (_Host(dtype=-1), M_), (_Host(g=0), N_), (_Host(g=66), -5),
+                      (_Host(n=(1 << 40) + 1), -6), (_Host(n=1 << 40), 0)):
+        if code:
+            assert bad.norm(P, P) == bad.clip(P, P, P) == bad.clip(None, P, P) == code and bad.bytes() == 0, code
+        else:
+            assert bad.bytes() > (1 << 40) // 4096 * 8
+    assert _Host(g=0, n=0).bytes() > 0
+    for fn, rest in ((lib.wq_grad_norm_list, (0, 1.0, P, P, None)), (lib.wq_grad_clip_list, (0, 1.0, 1.0, None, P, P, None))):
+        assert fn(None, None, None, 2, *rest) == N_ and fn(None, None, None, -1, *rest) == S
+        assert fn(good.keep[0], None, good.keep[2], 1, *rest) == N_
+    assert lib.wq_grad_clip_list(None, None, None, 0, 0, 1.0, 1.0, P, None, None, None) == 0                   # nothing to do
 
 
 def _hyper(**change):
@@ -270,9 +281,9 @@ def test_pieces_end_at_lines():
     assert per == _lib.ADAMW_ITEM and phase.tolist() == [31]
     for ptr in range(0, 128, 4):
         for n in (0, 1, 100, 4095, 4096, 4097, 12288):
-            t = torch.zeros(n)
-            count = 0 if n == 0 else -(-(n + ptr // 4) // 4096)
-            assert count <= optim._most_pieces(t)
+            host = _Host(g=1024 + ptr, n=n)
+            count = 1 + (0 if n == 0 else -(-(n + ptr // 4) // 4096))
+            assert host.bytes() == 64 + (count + 1) * 8
 
 
 def test_no_64_bit_shift_by_a_vector_register(tmp_path):
@@ -303,3 +314,36 @@ def test_no_64_bit_shift_by_a_vector_register(tmp_path):
     with concurrent.futures.ThreadPoolExecutor(max_workers=4) as pool:
         for src, found in pool.map(shifts, sorted(glob.glob(os.path.join(csrc, "*.hip")))):
             assert not found, (os.path.basename(src), found)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_list_workspace_is_large_enough(dtype):
+    """The bound that the host allocates by against the library's count, wherever the tensors start."""
+    size = torch.empty((), dtype=dtype).element_size()
+    for shift in range(0, 128, size):
+        for sizes in ([1], [4096, 8192], [1] * 300, [40960 * 3 + 1, 0, 7, 5_000_000], [0]):
+            n = (ctypes.c_int64 * len(sizes))(*sizes)
+            ptr = (ctypes.c_int64 * len(sizes))(*[(1 << 40) + shift] * len(sizes))
+            kind = (ctypes.c_int32 * len(sizes))(*[optim._DTYPES[dtype]] * len(sizes))
+            need = _lib.load().wq_grad_list_workspace_bytes(ptr, n, kind, len(sizes))
+            lst = optim._List.__new__(optim._List)
+            lst.n, lst.device = sizes, torch.device("cpu")
+            assert 0 < need <= lst.workspace().numel() * 8
+
+
+def test_list_overlaps():
+    for count in (3, 40):                        # the short form and the arrays
+        buf = torch.zeros(count * 10 + 10)
+        lst = optim._List.__new__(optim._List)
+
+        def check(ts):
+            lst.ptr, lst.n = (optim.array("q", [getattr(t, f)() for t in ts]) for f in ("data_ptr", "numel"))
+            lst.dtype = optim.array("i", [optim._DTYPES[t.dtype] for t in ts])
+            lst._refuse_overlaps("x")
+
+        ts = [buf[10 * i:10 * i + 10] for i in range(count)]
+        check(ts[::-1])
+        check(ts + [buf[5:5], buf[15:15]])
+        for more in (buf[:1], buf[count * 10 - 1:], ts[count // 2], buf):
+            with pytest.raises(ValueError, match="share memory"):
+                check(ts + [more])
