@@ -11,13 +11,19 @@
 
 namespace wq {
 
-// Both kernels: a workgroup takes 16 KiB of a gradient, four 16-byte loads per lane, all issued before the first use; an
-// unused dynamic LDS allocation caps the workgroups per CU.
-constexpr int kLoads = 4;
+// Norm: a workgroup takes a piece, four 16-byte loads per lane, all issued before the first use; an unused dynamic LDS
+// allocation caps the workgroups per CU.  A whole model's 14.5 GB of fp32 (3.6 G elements, 887 000 pieces): 1938 us = 7.5 TB/s
+// with 6 workgroups per CU; 8: 2015, 4: 2094, 3: 2499 us; plain instead of non-temporal loads: 2080 us.
+constexpr int kNormLoads = 4;
 constexpr int kNormPiecesPerXcdRun = 32;
 constexpr unsigned kNormOccupancyPadBytes = 27000;   // 6 workgroups per CU
-constexpr int kScalePiecesPerXcdRun = 32;
-constexpr unsigned kScaleOccupancyPadBytes = 40960;  // 4
+// Clip: half a piece per workgroup, two loads per lane.  604 M fp32 elements in place, norm included: 1050 us (of which the
+// norm is 320; 6.6 TB/s while it reads and writes); a whole piece and four loads with 4 workgroups per CU 1060, with 3 1167,
+// with 8 1103 us; one wavefront per workgroup with one load per lane 1076-1140 us.
+constexpr int kScaleLoads = 2;
+constexpr int kScaleParts = 2;
+constexpr int kScalePartsPerXcdRun = 64;
+constexpr unsigned kScaleOccupancyPadBytes = 20500;  // 7
 
 // ---- norm of a piece ------------------------------------------------------------------------------------------------
 template <int NORM, int D>
@@ -39,24 +45,24 @@ __device__ __forceinline__ u32x4 load_grad(const char* p) { return KEEP ? ldg16(
 template <int NORM, int D, bool KEEP>
 __device__ __forceinline__ typename NormAcc<NORM>::T piece_norm(const GradPiece& p)
 {
-    constexpr int kVec = 16 / dtype_bytes(D), kBatch = kLoads * kGradThreads;
+    constexpr int kVec = 16 / dtype_bytes(D), kBatch = kNormLoads * kGradThreads;
     typename NormAcc<NORM>::T a = NormAcc<NORM>::zero();
     const int t = threadIdx.x, head = head_of(p.g, dtype_bytes(D), p.n), whole = (p.n - head) / kVec;
     const char* g = p.g + head * dtype_bytes(D);
     for (int b = 0; b < whole; b += kBatch) {
-        u32x4 v[kLoads];
+        u32x4 v[kNormLoads];
         if (b + kBatch <= whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)(b + i * kGradThreads + t) * 16);
+            for (int i = 0; i < kNormLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)(b + i * kGradThreads + t) * 16);
         } else {  // lanes past the end load the last vector and count it as zeros
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
+            for (int i = 0; i < kNormLoads; ++i) v[i] = load_grad<KEEP>(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * 16);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
+            for (int i = 0; i < kNormLoads; ++i)
                 if (b + i * kGradThreads + t >= whole) v[i] = (u32x4){0u, 0u, 0u, 0u};
         }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) add_vec<NORM, D>(a, v[i]);
+        for (int i = 0; i < kNormLoads; ++i) add_vec<NORM, D>(a, v[i]);
     }
     if (t < head) NormAcc<NORM>::add(a, load_elem<D>(p.g, t));
     const int e = whole * kVec + t;
@@ -116,7 +122,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_each_kernel(const char
 }
 
 // ---- clip of a piece --------------------------------------------------------------------------------------------------
-// A lane takes the elements of one 16-byte access of the wider of the two types.
+// A lane takes the elements of one 16-byte access of the wider of the two types; part k of a piece's workgroups takes every
+// kScaleParts-th batch from batch k, the first one also what lies before the first 16-byte boundary and behind the last vector.
 template <int G, int O> struct ScaleVec {
     static constexpr int kElems = G == WQ_DTYPE_F32 || O == WQ_DTYPE_F32 ? 4 : 8;
     static constexpr int kIn = kElems * dtype_bytes(G), kOut = kElems * dtype_bytes(O);
@@ -150,50 +157,53 @@ template <int G, int O> struct ScaleVec {
     }
 };
 template <int G, int O>
-__device__ __forceinline__ void piece_scale(const GradPiece& p, float c)
+__device__ __forceinline__ void piece_scale(const GradPiece& p, int part, float c)
 {
     typedef ScaleVec<G, O> Vec;
-    constexpr int kBatch = kLoads * kGradThreads;
+    constexpr int kBatch = kScaleLoads * kGradThreads;
     constexpr int kG = dtype_bytes(G), kO = dtype_bytes(O);
     const int t = threadIdx.x, head = kO >= kG ? head_of(p.out, kO, p.n) : head_of(p.g, kG, p.n), n = p.n - head, whole = n / Vec::kElems;
     const char* g = p.g + head * kG;
     char* out = p.out + head * kO;
-    for (int b = 0; b < whole; b += kBatch) {
-        Vec v[kLoads];
+    for (int b = part * kBatch; b < whole; b += kScaleParts * kBatch) {
+        Vec v[kScaleLoads];
         if (b + kBatch <= whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].load(g + (size_t)(b + i * kGradThreads + t) * Vec::kIn);
+            for (int i = 0; i < kScaleLoads; ++i) v[i].load(g + (size_t)(b + i * kGradThreads + t) * Vec::kIn);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].scale_and_store(out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
+            for (int i = 0; i < kScaleLoads; ++i) v[i].scale_and_store(out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
         } else {  // lanes past the end load the last vector (in place perhaps as its owner stores it) and drop it
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i].load(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * Vec::kIn);
+            for (int i = 0; i < kScaleLoads; ++i) v[i].load(g + (size_t)min(b + i * kGradThreads + t, whole - 1) * Vec::kIn);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
+            for (int i = 0; i < kScaleLoads; ++i)
                 if (b + i * kGradThreads + t < whole) v[i].scale_and_store(out + (size_t)(b + i * kGradThreads + t) * Vec::kOut, c);
         }
     }
+    if (part) return;
     const int e = whole * Vec::kElems + t;
     if (e < n) store_elem<O>(out, e, load_elem<G>(g, e) * c);
     if (t < head) store_elem<O>(p.out, t, load_elem<G>(p.g, t) * c);
 }
 template <int G>
-__device__ __forceinline__ void piece_scale_from(const GradPiece& p, float c)
+__device__ __forceinline__ void piece_scale_from(const GradPiece& p, int part, float c)
 {
-    if (p.out_dtype == WQ_DTYPE_BF16) piece_scale<G, WQ_DTYPE_BF16>(p, c);
-    else if (p.out_dtype == WQ_DTYPE_F16) piece_scale<G, WQ_DTYPE_F16>(p, c);
-    else piece_scale<G, WQ_DTYPE_F32>(p, c);
+    if (p.out_dtype == WQ_DTYPE_BF16) piece_scale<G, WQ_DTYPE_BF16>(p, part, c);
+    else if (p.out_dtype == WQ_DTYPE_F16) piece_scale<G, WQ_DTYPE_F16>(p, part, c);
+    else piece_scale<G, WQ_DTYPE_F32>(p, part, c);
 }
 
 // NORM < 0: the norm is at `total`.  Otherwise every workgroup folds the list's partials for itself - kFoldByAll at most, a
 // microsecond - in the order in which the total's kernel would, and the first one writes the norm: a launch less where the
 // launches are most of the time (router and norm vectors of a layer: 3 -> 2).
 template <int NORM, typename Source>
-__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_items, float* total, float max_norm,
+__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_parts, float* total, float max_norm,
                                                                  float scale, const float* scale_dev, const Partials partials)
 {
     const int64_t slot = (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-    GradPiece p = src.piece(item_of_slot(slot, n_items, kScalePiecesPerXcdRun));
+    const int64_t unit = item_of_slot(slot, n_parts, kScalePartsPerXcdRun);
+    const int part = (int)(unit % kScaleParts);
+    GradPiece p = src.piece(unit / kScaleParts);
     uint32_t norm_bits = NORM < 0 ? const_u32(total) : 0u, dev = 0u;
     if (NORM < 0) dev = const_u32(scale_dev ? scale_dev : total);
     else if (scale_dev) dev = const_u32(scale_dev);
@@ -206,10 +216,10 @@ __global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source s
         if (slot == 0 && threadIdx.x == 0) stg<float>(total, norm);
     }
     const float c = clip_coefficient(norm, max_norm, s);
-    if (slot >= n_items || (c == 1.0f && p.out == p.g)) return;  // uniform per workgroup
-    if (p.g_dtype == WQ_DTYPE_BF16) piece_scale_from<WQ_DTYPE_BF16>(p, c);
-    else if (p.g_dtype == WQ_DTYPE_F16) piece_scale_from<WQ_DTYPE_F16>(p, c);
-    else piece_scale_from<WQ_DTYPE_F32>(p, c);
+    if (slot >= n_parts || (c == 1.0f && p.out == p.g)) return;  // uniform per workgroup
+    if (p.g_dtype == WQ_DTYPE_BF16) piece_scale_from<WQ_DTYPE_BF16>(p, part, c);
+    else if (p.g_dtype == WQ_DTYPE_F16) piece_scale_from<WQ_DTYPE_F16>(p, part, c);
+    else piece_scale_from<WQ_DTYPE_F32>(p, part, c);
 }
 
 // ---- per-tensor descriptors -> one per piece ----------------------------------------------------------------------------
@@ -302,8 +312,9 @@ static void launch_scale(const Source& src, int64_t n_items, float* total, float
                          Partials partials, hipStream_t st)
 {
     if (n_items == 0) return;
-    grad_scale_kernel<NORM><<<grid_for_items(n_items), kGradThreads, kScaleOccupancyPadBytes, st>>>(src, n_items, total, max_norm, scale,
-                                                                                                    scale_dev, partials);
+    const int64_t parts = n_items * kScaleParts;
+    grad_scale_kernel<NORM><<<grid_for_items(parts), kGradThreads, kScaleOccupancyPadBytes, st>>>(src, parts, total, max_norm, scale,
+                                                                                                   scale_dev, partials);
 }
 template <int NORM>
 static void launch_table_clip(const TableSource& src, int64_t n_items, float max_norm, float scale, const float* scale_dev,

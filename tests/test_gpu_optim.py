@@ -392,6 +392,22 @@ def test_adamw_from_fresh_state_follows_torch(cuda):
     assert plan.step.item() == 10
 
 
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.0, 0.0), (0.5, 0.0), (0.9999999, 0.99999999)])
+@pytest.mark.parametrize("step", [0, 1, 99, 123456789])
+def test_adamw_bias_corrections(cuda, betas, step):
+    """Early, late and degenerate corrections, which the device forms in 64 bits: the first moment's is seen in the step of an
+    element whose moments are steady."""
+    b1, b2 = betas
+    p, m, v, g = ([torch.full((9,), x, device=cuda)] for x in (0.0, 0.5, 0.25, 0.5))
+    plan = slime_amd.AdamWPlan(p, g, None, m, v, betas=betas, eps=0.0, weight_decay=0.0, step=step)
+    plan.run(1.0)
+    t = step + 1
+    want = -(1 - b2 ** t) ** 0.5 / (1 - b1 ** t)
+    # fp32 (1 - beta) is exact to u of its own size; moments, root, division and the two step constants: under 16 roundings
+    assert abs(p[0][0].item() - want) <= 16 * U * abs(want), (p[0][0].item(), want)
+    assert plan.step.item() == t
+
+
 def test_adamw_zero_gradients_and_state(cuda):
     p = torch.randn(ITEM + 9, device=cuda)
     g = torch.zeros_like(p)
