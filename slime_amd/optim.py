@@ -8,7 +8,7 @@ the clip as a factor (no pass of its own) and writes the bf16 / fp16 weight that
 ``get_total_norm``, ``clip_grad_norm_`` and ``clip_grads_with_norm_`` have the names and arguments of ``torch.nn.utils`` and take
 whatever gradients a call presents; ``GradNormPlan``, ``GradClipPlan`` and ``AdamWPlan`` take a fixed list (gradient buffers that
 stay where they are) and can be captured into a HIP graph.  Norms are fp32, whatever the gradients' type: sums of squares are
-formed in 64 bits in a fixed order, so they neither overflow nor depend on the run.
+formed in 64 bits in a fixed order, so they neither overflow nor depend on the run (a norm beyond fp32's range is infinite).
 
 Norm of a model that is sharded over ranks: ``norm = plan.run(); total = norm.square(); all_reduce(total);`` and
 ``total_norm=total.sqrt()`` in the clip or the update.
@@ -17,6 +17,7 @@ Norm of a model that is sharded over ranks: ``norm = plan.run(); total = norm.sq
 from __future__ import annotations
 
 import math
+import numbers
 from array import array
 from contextlib import nullcontext
 from typing import Iterable, Sequence
@@ -49,8 +50,9 @@ def _check_tensor(t, what: str, dtypes=_DTYPES) -> None:
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
     if t.layout != torch.strided or hasattr(t, "to_local"):
         raise TypeError(f"{what}: only plain strided tensors are supported (of a sharded one, pass the local part)")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{what}: dtype {t.dtype} is not supported ({', '.join(str(d) for d in dtypes)})")
+    if t.dtype not in dtypes or t.is_neg():
+        raise TypeError(f"{what}: dtype {t.dtype}{' with a pending negation' * t.is_neg()} is not supported "
+                        f"({', '.join(str(d) for d in dtypes)})")
 
 
 def _strides(t):
@@ -163,8 +165,11 @@ def _cuts(rows: np.ndarray):
 def _item_table(rows: np.ndarray, device, what: str):
     """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
     of the tensors in it, number of items)."""
-    starts = np.zeros(len(rows) + 1, dtype=np.int64)
     n = rows[:, 2]
+    g, out = (np.where(d == _lib.DTYPE_F32, 4, 2) for d in (rows[:, 3] & 0xFFFFFFFF, rows[:, 3] >> 32))
+    if (rows[:, 0] % g).any() or (rows[:, 1] % out).any() or (rows[:, 4:7] % 4).any():
+        raise ValueError(f"{what}: a tensor does not start at a multiple of its element size")
+    starts = np.zeros(len(rows) + 1, dtype=np.int64)
     per, phase = _cuts(rows)
     np.cumsum(np.where(n > 0, -(-(n + phase) // per), 0), out=starts[1:])
     table = torch.from_numpy(np.concatenate([rows.reshape(-1), starts])).to(device)
@@ -176,8 +181,9 @@ def _item_table(rows: np.ndarray, device, what: str):
 
 
 class _Plan:
-    """Tables and workspace of a fixed list.  One plan's runs must be ordered on one stream (or by events): they share the
-    workspace.  A run on another stream than the one the plan was built on is fine."""
+    """Tables and workspace of a fixed list.  One plan's runs - captured ones too - must be ordered on one stream (or by
+    events): they share the workspace and the result.  The stream need not be the one the plan was built on.  The plan reads
+    and writes the tensors it was given, wherever their contents come from; one that moves needs a new plan."""
 
     def _build(self, rows, device, what: str) -> None:
         self.device, self._what = device, what
@@ -244,8 +250,9 @@ class GradClipPlan(_Plan):
     with ``out``, into other tensors of the same shapes and layouts (bf16 gradients into fp32 main gradients, say), rounded
     once.  In place, gradients that need no change are not rewritten.
 
-    ``run(max_norm, grad_scale=1.0, total_norm=None)`` returns the norm before the clip (of the scaled gradients): a 0-d fp32
-    tensor that the next run overwrites, or the ``total_norm`` it was given."""
+    ``run(max_norm, grad_scale=1.0, total_norm=None)`` returns the norm before the clip: a 0-d fp32 tensor that the next run
+    overwrites.  ``total_norm`` (one fp32 value on the device, of the gradients times grad_scale) is taken for the norm, and
+    returned, if it is given."""
 
     def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, out: Sequence[torch.Tensor] | None = None):
         self._norm = _norm_selector(norm_type, "GradClipPlan")
@@ -274,7 +281,7 @@ class GradClipPlan(_Plan):
 
 
 def _per_tensor(value, n: int, what: str):
-    values = [float(value)] * n if isinstance(value, (int, float)) else [float(v) for v in value]
+    values = [float(value)] * n if isinstance(value, numbers.Real) else [float(v) for v in value]
     if len(values) != n:
         raise ValueError(f"AdamWPlan: need one {what} per parameter")
     for v in values:
@@ -312,14 +319,12 @@ class AdamWPlan(_Plan):
             raise ValueError(f"AdamWPlan: step must not be negative, got {step}")
         self.grads, self.params = _check_grads(grads, "AdamWPlan"), list(params)
         n = len(self.params)
-        self.weights = [None] * n if weights is None else list(weights)
-        given = [self.params, self.grads, self.weights] + [list(x) for x in (exp_avgs, exp_avg_sqs) if x is not None]
-        if any(len(x) != n for x in given):
+        self.weights, *moments = ([None] * n if x is None else list(x) for x in (weights, exp_avgs, exp_avg_sqs))
+        if any(len(x) != n for x in (self.grads, self.weights, *moments)):
             raise ValueError("AdamWPlan: need equally many parameters, gradients, weights and moments")
         decay, lr_scales = _per_tensor(weight_decay, n, "weight_decay"), _per_tensor(lr_scale, n, "lr_scale")
         for p in self.params:
             _check_tensor(p, "AdamWPlan: parameters", (torch.float32,))
-        moments = [[None] * n if x is None else list(x) for x in (exp_avgs, exp_avg_sqs)]
         for p, g, w, m, v in zip(self.params, self.grads, self.weights, *moments):
             for x in (m, v):
                 if x is not None:

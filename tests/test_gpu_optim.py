@@ -570,6 +570,70 @@ def test_a_training_step_as_it_is_used(cuda):
             assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(sc, sc2)
 
 
+def test_inference_tensors_and_saved_tensors(cuda):
+    """Tensors without a version counter work; autograd refuses a backward through what a clip has overwritten."""
+    with torch.inference_mode():
+        t = torch.ones(100, device=cuda)
+        p = torch.nn.Parameter(torch.zeros(100, device=cuda), requires_grad=False)
+    p.grad = t
+    assert abs(slime_amd.clip_grad_norm_(p, 1.0).item() - 10.0) < 1e-5 and abs(t[0].item() - 0.1) < 1e-6
+    slime_amd.GradClipPlan([t]).run(0.5)
+    assert abs(t[0].item() - 0.05) < 1e-6
+    x = torch.ones(10, device=cuda, requires_grad=True)
+    g = torch.full((10,), 3.0, device=cuda)
+    y = (x * g).sum()                                       # saves g
+    slime_amd.GradClipPlan([g]).run(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
+def test_calls_from_two_threads_on_streams_of_their_own(cuda):
+    import threading
+
+    lists = [tensors([(1000, 37 + i), (5,), (ITEM * 3 + i,)] * 20, [BF16, F32], 80 + i, 1.0 + i) for i in range(2)]
+    want = [norm_of(ts) for ts in lists]
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            plan = slime_amd.GradNormPlan(lists[i], per_tensor=True)
+            for k in range(30):
+                a, b = slime_amd.get_total_norm(lists[i]), plan.run()[0]
+                if abs(a.item() - want[i]) > 2 * U * want[i] or abs(b.item() - want[i]) > 2 * U * want[i]:
+                    bad.append((i, k, a.item(), b.item()))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_two_graphs_of_one_plan_replayed_in_turn(cuda):
+    ts = tensors([(ITEM * 2 + 3,), (77, 5)], [BF16], 90)
+    norm, clip = slime_amd.GradNormPlan(ts), slime_amd.GradClipPlan(ts)
+    side, graphs = torch.cuda.Stream(), []
+    side.wait_stream(torch.cuda.current_stream())
+    for max_norm in (3.0, 1.0):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.stream(side), torch.cuda.graph(graphs[-1], stream=side):
+            norm.run()
+            clip.run(max_norm)
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(4):
+        for t in ts:
+            t.normal_()
+        before = [t.clone() for t in ts]
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert abs(norm.total_norm.item() - 3.0) < 1e-2 and abs(norm_of(ts) - 1.0) < 1e-2       # bf16 roundings average out
+        assert all(((t.double() - b.double() / norm_of(before)).abs() <= b.double().abs() / norm_of(before) * 2.0 ** -6).all() for t, b in zip(ts, before))
+
+
 def test_item_tables_are_exact(cuda):
     """Every row of a table of half a million pieces, from tensors of mixed types and starts (a per-lane 64-bit shift went wrong in
     one wavefront of a hundred here)."""

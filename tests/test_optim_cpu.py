@@ -127,6 +127,32 @@ def test_plans_refuse(plan):
         plan([torch.zeros(4, 1).expand(4, 8)])
 
 
+def test_what_a_plan_cannot_read_as_it_lies():
+    neg = torch.zeros(4, 8, dtype=torch.complex64).conj().imag
+    flipped = torch._neg_view(torch.zeros(4, 8))
+    assert neg.is_neg() and flipped.is_neg()
+    for plan in PLANS:
+        with pytest.raises(TypeError, match="negation"):
+            plan([flipped])
+    odd = np.array([[1025, 1024, 4, 0], [1024, 1025, 4, 0], [1026, 1024, 4, 1], [1024, 1026, 4, 1 << 32]], dtype=np.int64)
+    for row in odd:
+        with pytest.raises(ValueError, match="multiple of its element"):
+            optim._item_table(row[None], torch.device("cpu"), "x")
+    for k in (4, 5, 6):
+        row = np.array([[1024, 0, 4, 0, 1024, 1024, 1024, 0]], dtype=np.int64)
+        row[0, k] += 2
+        with pytest.raises(ValueError, match="multiple of its element"):
+            optim._item_table(row, torch.device("cpu"), "x")
+
+
+def test_lists_may_be_iterators_and_numbers_numpy_ones():
+    with pytest.raises(RuntimeError, match="GPU"):
+        optim.AdamWPlan(iter(_lists()), iter(_lists()), iter([None, None, None]), iter(_lists()), iter(_lists()),
+                        weight_decay=np.float32(0.1), lr_scale=np.ones(3))
+    with pytest.raises(RuntimeError, match="GPU"):
+        optim.GradClipPlan(iter(_lists()), out=iter(_lists()))
+
+
 @pytest.mark.parametrize("call", [lambda g: slime_amd.get_total_norm(g), lambda g: slime_amd.get_total_norm(g[0]),
                                   lambda g: slime_amd.clip_grad_norm_(_params(g), 1.0),
                                   lambda g: slime_amd.clip_grad_norm_(_params(g)[0], 1.0, error_if_nonfinite=True),
