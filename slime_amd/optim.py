@@ -30,6 +30,12 @@ from . import _lib
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 _NORMS = {2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 
+# Lists of hundreds of tensors are looked at by passes that stay in C, map() over these (40 ns a tensor); only where something is
+# out of the ordinary are they looked at one by one.
+_data_ptr, _numel, _is_contiguous, _get_device, _is_neg = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device", "is_neg"))
+_dtype, _layout, _shape, _nbytes = (getattr(torch.Tensor, n).__get__ for n in ("dtype", "layout", "shape", "nbytes"))
+_PLAIN_TYPES = {torch.Tensor, torch.nn.Parameter}
+
 
 def _norm_selector(norm_type, what: str) -> int:
     norm = _NORMS.get(float(norm_type))
@@ -53,6 +59,14 @@ def _check_tensor(t, what: str, dtypes=_DTYPES) -> None:
     if t.dtype not in dtypes or t.is_neg():
         raise TypeError(f"{what}: dtype {t.dtype}{' with a pending negation' * t.is_neg()} is not supported "
                         f"({', '.join(str(d) for d in dtypes)})")
+
+
+def _check_tensors(tensors, what: str, dtypes=_DTYPES) -> None:
+    if set(map(type, tensors)) <= _PLAIN_TYPES and set(map(_layout, tensors)) <= {torch.strided} and \
+            set(map(_dtype, tensors)) <= set(dtypes) and not any(map(_is_neg, tensors)):
+        return
+    for t in tensors:
+        _check_tensor(t, what, dtypes)
 
 
 def _strides(t):
@@ -85,27 +99,35 @@ def _same_layout(a, b) -> bool:
                                    all(n == 1 or x == y for x, y, n in zip(a.stride(), b.stride(), a.shape)))
 
 
+def _same_layouts(tensors, others) -> bool:
+    if all(map(_is_contiguous, tensors)) and all(map(_is_contiguous, others)):
+        return all(map(torch.Size.__eq__, map(_shape, tensors), map(_shape, others)))
+    return all(map(_same_layout, tensors, others))
+
+
 def _one_device(tensors, what: str) -> torch.device:
-    device = tensors[0].device
+    indices = set(map(_get_device, tensors))
+    if len(indices) == 1 and min(indices) >= 0:
+        return tensors[0].device
     for t in tensors:
         _lib.require_gpu(t, what)
-        if t.device != device:
-            raise ValueError(f"{what}: all tensors must be on one device (got {device} and {t.device})")
-    return device
+    raise ValueError(f"{what}: all tensors must be on one device (got {sorted(set(str(t.device) for t in tensors))})")
+
+
+def _column(f, tensors) -> np.ndarray:
+    return np.fromiter(map(f, tensors), dtype=np.int64, count=len(tensors))
 
 
 def _refuse_overlaps(written, read, what: str) -> None:
     """Ranges that are written share no byte with each other or with one that is read."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w)
-             for ts, w in ((written, True), (read, False)) for t in ts if t.numel()]
-    if not spans:
-        return
-    a = np.array(spans, dtype=np.int64)
-    a = a[np.lexsort((a[:, 1], a[:, 0]))]
-    end, w = a[:, 1], a[:, 2].astype(bool)
+    tensors = [*written, *read]
+    start, size = _column(_data_ptr, tensors), _column(_nbytes, tensors)
+    w = np.arange(len(tensors)) < len(written)
+    order = np.argsort(start[size > 0], kind="stable")
+    start, end, w = (x[size > 0][order] for x in (start, start + size, w))
     any_end = np.maximum.accumulate(end)[:-1]
     written_end = np.maximum.accumulate(np.where(w, end, 0))[:-1]
-    if ((a[1:, 0] < written_end) | (w[1:] & (a[1:, 0] < any_end))).any():
+    if ((start[1:] < written_end) | (w[1:] & (start[1:] < any_end))).any():
         raise ValueError(f"{what}: tensors that are written share memory with others of the call (the same tensor twice?)")
 
 
@@ -148,9 +170,9 @@ def _workspace(n_items: int, device) -> torch.Tensor:
     return torch.empty(_lib.load().wq_grad_workspace_bytes(n_items) // 8, dtype=torch.int64, device=device)
 
 
-def _grad_row(g, out=None):
-    out = g if out is None else out
-    return [g.data_ptr(), out.data_ptr(), g.numel(), _DTYPES[g.dtype] | _DTYPES[out.dtype] << 32]
+def _grad_rows(grads, outs) -> np.ndarray:
+    kind = _column(_DTYPES.get, list(map(_dtype, grads))) | _column(_DTYPES.get, list(map(_dtype, outs))) << 32
+    return np.stack([_column(_data_ptr, grads), _column(_data_ptr, outs), _column(_numel, grads), kind], axis=1)
 
 
 def _cuts(rows: np.ndarray):
@@ -188,7 +210,7 @@ class _Plan:
     def _build(self, rows, device, what: str) -> None:
         self.device, self._what = device, what
         with torch.cuda.device(device):
-            self._items, self._starts, self._n_items = _item_table(np.array(rows, dtype=np.int64), device, what)
+            self._items, self._starts, self._n_items = _item_table(rows, device, what)
             self._workspace = _workspace(self._n_items, device)
             self.total_norm = torch.zeros((), dtype=torch.float32, device=device)
             self._stream = torch.cuda.current_stream(device)
@@ -212,8 +234,8 @@ def _check_grads(grads, what: str):
     grads = list(grads)
     if not grads:
         raise ValueError(f"{what}: empty gradient list")
-    for g in grads:
-        _check_tensor(g, what)
+    _check_tensors(grads, what)
+    for g in grads if not all(map(_is_contiguous, grads)) else ():
         if not _is_dense(g):
             raise ValueError(f"{what}: tensors of a plan must fill one run of memory (a copy would be read instead of the live "
                              f"gradient); got shape {tuple(g.shape)}, strides {tuple(g.stride())}")
@@ -230,7 +252,7 @@ class GradNormPlan(_Plan):
     def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_tensor: bool = False):
         self._norm = _norm_selector(norm_type, "GradNormPlan")
         self.grads = _check_grads(grads, "GradNormPlan")
-        self._build([_grad_row(g) for g in self.grads], _one_device(self.grads, "GradNormPlan"), "GradNormPlan")
+        self._build(_grad_rows(self.grads, self.grads), _one_device(self.grads, "GradNormPlan"), "GradNormPlan")
         self.norms = torch.zeros(len(self.grads), dtype=torch.float32, device=self.device) if per_tensor else None
         if per_tensor:
             self._owned.append(self.norms)
@@ -260,15 +282,14 @@ class GradClipPlan(_Plan):
         self.out = self.grads if out is None else list(out)
         if len(self.out) != len(self.grads):
             raise ValueError("GradClipPlan: need one output per gradient")
-        for g, o in zip(self.grads, self.out):
-            _check_tensor(o, "GradClipPlan")
-            if not _same_layout(g, o):
-                raise ValueError(f"GradClipPlan: output of shape {tuple(o.shape)}, strides {tuple(o.stride())} for a gradient of "
-                                 f"shape {tuple(g.shape)}, strides {tuple(g.stride())}")
-        apart = [g for g, o in zip(self.grads, self.out) if g.data_ptr() != o.data_ptr() or g.dtype != o.dtype]
+        _check_tensors(self.out, "GradClipPlan")
+        if not _same_layouts(self.grads, self.out):
+            g, o = next((g, o) for g, o in zip(self.grads, self.out) if not _same_layout(g, o))
+            raise ValueError(f"GradClipPlan: output of shape {tuple(o.shape)}, strides {tuple(o.stride())} for a gradient of "
+                             f"shape {tuple(g.shape)}, strides {tuple(g.stride())}")
+        apart = [g for g, o in zip(self.grads, self.out) if g is not o and (g.data_ptr() != o.data_ptr() or g.dtype != o.dtype)]
         _refuse_overlaps(self.out, apart, "GradClipPlan")
-        device = _one_device(self.grads + self.out, "GradClipPlan")
-        self._build([_grad_row(g, o) for g, o in zip(self.grads, self.out)], device, "GradClipPlan")
+        self._build(_grad_rows(self.grads, self.out), _one_device(self.grads + self.out, "GradClipPlan"), "GradClipPlan")
         self._built()
 
     def run(self, max_norm: float, grad_scale=1.0, total_norm: torch.Tensor | None = None) -> torch.Tensor:
@@ -323,17 +344,17 @@ class AdamWPlan(_Plan):
         if any(len(x) != n for x in (self.grads, self.weights, *moments)):
             raise ValueError("AdamWPlan: need equally many parameters, gradients, weights and moments")
         decay, lr_scales = _per_tensor(weight_decay, n, "weight_decay"), _per_tensor(lr_scale, n, "lr_scale")
-        for p in self.params:
-            _check_tensor(p, "AdamWPlan: parameters", (torch.float32,))
-        for p, g, w, m, v in zip(self.params, self.grads, self.weights, *moments):
-            for x in (m, v):
-                if x is not None:
-                    _check_tensor(x, "AdamWPlan: moments", (torch.float32,))
-            if w is not None:
-                _check_tensor(w, "AdamWPlan: weights", (torch.bfloat16, torch.float16))
-            if not all(_same_layout(p, x) for x in (g, w, m, v) if x is not None):
+        _check_tensors(self.params, "AdamWPlan: parameters", (torch.float32,))
+        given = {"moments": ((torch.float32,), moments), "weights": ((torch.bfloat16, torch.float16), [self.weights])}
+        for name, (dtypes, lists) in given.items():
+            for xs in lists:
+                _check_tensors([x for x in xs if x is not None], f"AdamWPlan: {name}", dtypes)
+        for xs in (self.grads, self.weights, *moments):
+            pairs = [(p, x) for p, x in zip(self.params, xs) if x is not None]
+            if pairs and not _same_layouts(*zip(*pairs)):
+                p, x = next(pair for pair in pairs if not _same_layout(*pair))
                 raise ValueError(f"AdamWPlan: gradient, weight and moments must have the shape and strides of their parameter "
-                                 f"({tuple(p.shape)}, {tuple(p.stride())})")
+                                 f"(got {tuple(x.shape)}, {tuple(x.stride())} for {tuple(p.shape)}, {tuple(p.stride())})")
         self._written = self.params + [w for w in self.weights if w is not None]
         state = [x for xs in moments for x in xs if x is not None]
         _refuse_overlaps(self._written + state, self.grads, "AdamWPlan")
@@ -342,10 +363,15 @@ class AdamWPlan(_Plan):
         moments = [[torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=device).zero_() if x is None else x
                     for p, x in zip(self.params, xs)] for xs in moments]
         self.exp_avgs, self.exp_avg_sqs = moments
-        floats = np.array([lr_scales, decay], dtype=np.float32).T.copy().view(np.int64).reshape(-1)
-        rows = [[g.data_ptr(), 0 if w is None else w.data_ptr(), p.numel(), _DTYPES[g.dtype] | (0 if w is None else _DTYPES[w.dtype]) << 32,
-                 p.data_ptr(), m.data_ptr(), v.data_ptr(), int(f)]
-                for p, g, w, m, v, f in zip(self.params, self.grads, self.weights, self.exp_avgs, self.exp_avg_sqs, floats)]
+        rows = np.zeros((n, 8), dtype=np.int64)
+        rows[:, :4] = _grad_rows(self.grads, self.grads)
+        has = np.array([w is not None for w in self.weights])
+        rows[:, 1], rows[:, 3] = 0, rows[:, 3] & 0xFFFFFFFF
+        rows[has, 1] = _column(_data_ptr, [w for w in self.weights if w is not None])
+        rows[has, 3] |= _column(_DTYPES.get, [w.dtype for w in self.weights if w is not None]) << 32
+        for k, xs in enumerate((self.params, self.exp_avgs, self.exp_avg_sqs)):
+            rows[:, 4 + k] = _column(_data_ptr, xs)
+        rows[:, 7] = np.array([lr_scales, decay], dtype=np.float32).T.copy().view(np.int64)[:, 0]
         self._build(rows, device, "AdamWPlan")
         self.skip_nonfinite = bool(skip_nonfinite)
         self.step = torch.full((), int(step), dtype=torch.int64, device=device)
@@ -375,11 +401,6 @@ def _grads_of(parameters) -> list:
     return [g for p in parameters if (g := p.grad) is not None]
 
 
-_data_ptr, _numel, _is_contiguous, _get_device = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device"))
-_dtype = torch.Tensor.dtype.__get__
-_PLAIN_TYPES = {torch.Tensor, torch.nn.Parameter}
-
-
 class _List:
     """Tensors as the list entry points take them: host arrays of addresses, element counts and types.  The common case -
     contiguous tensors of one GPU - is found out by passes that stay in C (0.2 us a tensor); anything else is looked at
@@ -406,8 +427,7 @@ class _List:
         self.args = (self.ptr.buffer_info()[0], self.n.buffer_info()[0], self.dtype.buffer_info()[0], len(tensors))
 
     def _one_by_one(self, tensors, what: str, written: bool):
-        for t in tensors:
-            _check_tensor(t, what)
+        _check_tensors(tensors, what)
         self.index = _one_device(tensors, what).index
         dense = []
         for t in tensors:
