@@ -3,7 +3,7 @@
 //   norm_2 = s * sqrt(sum g^2), norm_inf = s * max |g|, coefficient = s * min(1, max_norm / (norm + 1e-6)), out = round(g * c)
 //
 // Both are bound by HBM: the norm reads every gradient once, the clip reads it again and writes it.  One workgroup takes one
-// piece of at most 16384 elements of one tensor and leaves one 64-bit partial; a fold of the partials in a fixed order
+// piece, 16 KiB of one tensor, and leaves one 64-bit partial; a fold of the partials in a fixed order
 // gives the norm (no atomics, so the same gradients give the same bits).  Squares are added in 64 bits: fp32 squares are
 // exact there and can neither overflow nor vanish.
 
@@ -13,7 +13,7 @@ namespace wq {
 
 // Norm: a workgroup takes a piece, four 16-byte loads per lane, all issued before the first use; an unused dynamic LDS
 // allocation caps the workgroups per CU.  A whole model's 14.5 GB of fp32 (3.6 G elements, 887 000 pieces): 1938 us = 7.5 TB/s
-// with 6 workgroups per CU; 8: 2015, 4: 2094, 3: 2499 us; plain instead of non-temporal loads: 2080 us.
+// with 6 workgroups per CU; 8: 2015, 4: 2094, 3: 2499 us.
 constexpr int kNormLoads = 4;
 constexpr int kNormPiecesPerXcdRun = 32;
 constexpr unsigned kNormOccupancyPadBytes = 27000;   // 6 workgroups per CU
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
 
 // A norm whose gradients are read again right away (`again`) leaves them in the 256 MB Infinity Cache if they fit: plain
 // instead of non-temporal loads make the norm alone slower (202 MB of bf16: 35 -> 38 us) and norm and clip together faster
-// (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 87 -> 81 us); with 2.4 GB nothing is left to find (1060 -> 1087 us).
+// (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 83 -> 80 us); with 2.4 GB nothing is left to find (1060 -> 1087 us).
 constexpr int64_t kKeepPieces = (256 << 20) / WQ_GRAD_ITEM_BYTES;
 
 template <int NORM, typename Source>

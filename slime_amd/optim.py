@@ -226,6 +226,12 @@ class _Plan:
                 t.record_stream(stream)
         _launch(self.device, entry, self._what, *args)
 
+    def _factor(self, value, what: str):
+        factor, address = _scale_args(value, self.device, f"{self._what}: {what}")
+        if address is not None and address == self.total_norm.data_ptr():
+            raise ValueError(f"{self._what}: {what} must not be the plan's own total_norm, which the run overwrites")
+        return factor, address
+
     def _given(self, total_norm):
         return None if total_norm is None else _scalar_on_device(total_norm, self.device, f"{self._what}: total_norm")
 
@@ -259,7 +265,7 @@ class GradNormPlan(_Plan):
         self._built()
 
     def run(self, grad_scale=1.0):
-        scale, scale_dev = _scale_args(grad_scale, self.device, "GradNormPlan: grad_scale")
+        scale, scale_dev = self._factor(grad_scale, "grad_scale")
         each = self.norms
         self._run("wq_grad_norm_items", self._items.data_ptr(), self._n_items, 4, self._starts.data_ptr(), len(self.grads),
                   self._norm, scale, scale_dev, self._workspace.data_ptr(), self.total_norm.data_ptr(),
@@ -294,7 +300,7 @@ class GradClipPlan(_Plan):
 
     def run(self, max_norm: float, grad_scale=1.0, total_norm: torch.Tensor | None = None) -> torch.Tensor:
         max_norm = _check_max_norm(max_norm, "GradClipPlan")
-        scale, scale_dev = _scale_args(grad_scale, self.device, "GradClipPlan: grad_scale")
+        scale, scale_dev = self._factor(grad_scale, "grad_scale")
         self._run("wq_grad_clip_items", self._items.data_ptr(), self._n_items, self._norm, max_norm, scale, scale_dev,
                   self._given(total_norm), self._workspace.data_ptr(), self.total_norm.data_ptr())
         _bump(self.out)
@@ -359,9 +365,12 @@ class AdamWPlan(_Plan):
         state = [x for xs in moments for x in xs if x is not None]
         _refuse_overlaps(self._written + state, self.grads, "AdamWPlan")
         device = _one_device(self.params + self.grads + self._written + state, "AdamWPlan")
-        # fresh moments in the parameter's layout
-        moments = [[torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=device).zero_() if x is None else x
-                    for p, x in zip(self.params, xs)] for xs in moments]
+        fresh = []
+        for xs in moments:
+            for i, p in enumerate(self.params):
+                if xs[i] is None:           # in the parameter's layout
+                    xs[i] = torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=device).zero_()
+                    fresh.append(xs[i])
         self.exp_avgs, self.exp_avg_sqs = moments
         rows = np.zeros((n, 8), dtype=np.int64)
         rows[:, :4] = _grad_rows(self.grads, self.grads)
@@ -375,7 +384,7 @@ class AdamWPlan(_Plan):
         self._build(rows, device, "AdamWPlan")
         self.skip_nonfinite = bool(skip_nonfinite)
         self.step = torch.full((), int(step), dtype=torch.int64, device=device)
-        self._owned.append(self.step)
+        self._owned += [self.step, *fresh]
         self._hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, 0.0, None, None, None, self.total_norm.data_ptr(),
                                       self.step.data_ptr(), 1.0, -1.0, self._norm, self.skip_nonfinite)
         self._built()
@@ -383,8 +392,8 @@ class AdamWPlan(_Plan):
     def run(self, lr, max_norm: float | None = None, grad_scale=1.0, total_norm: torch.Tensor | None = None):
         max_norm = -1.0 if max_norm is None else _check_max_norm(max_norm, "AdamWPlan")
         h = self._hyper
-        h.lr, h.lr_dev = _scale_args(lr, self.device, "AdamWPlan: lr")
-        h.grad_scale, h.grad_scale_dev = _scale_args(grad_scale, self.device, "AdamWPlan: grad_scale")
+        h.lr, h.lr_dev = self._factor(lr, "lr")
+        h.grad_scale, h.grad_scale_dev = self._factor(grad_scale, "grad_scale")
         h.total_given, h.max_norm = self._given(total_norm), max_norm
         self._run("wq_adamw_items", self._items.data_ptr(), self._n_items, h, self._workspace.data_ptr())
         _bump(self._written)

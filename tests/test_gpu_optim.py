@@ -455,6 +455,12 @@ def test_adamw_device_scalars_and_given_norm(cuda):
         assert all(torch.equal(x, y) for x, y in zip(xs, ys))
     with pytest.raises(ValueError, match="lr"):
         pa.run(torch.tensor(0.1))
+    for call in (lambda: pa.run(0.1, grad_scale=pa.total_norm), lambda: pa.run(pa.total_norm)):
+        with pytest.raises(ValueError, match="own total_norm"):
+            call()
+    for plan in (slime_amd.GradNormPlan(a[3]), slime_amd.GradClipPlan(a[3])):
+        with pytest.raises(ValueError, match="own total_norm"):
+            plan.run(*([1.0] if isinstance(plan, slime_amd.GradClipPlan) else []), grad_scale=plan.total_norm)
 
 
 def test_adamw_any_dense_layout_and_fresh_moments(cuda):
