@@ -331,7 +331,8 @@ class AdamWPlan(_Plan):
     replays.  With ``skip_nonfinite`` a step whose gradient norm is infinite or NaN changes nothing and is not counted.
 
     ``run(lr, max_norm=None, grad_scale=1.0, total_norm=None)``: lr is a number or one fp32 value on the device (a number is
-    fixed in a captured run).  Returns the gradient norm before the clip where it is needed (max_norm or skip_nonfinite; a 0-d
+    fixed in a captured run).  Parameters with other betas are a plan of their own; the norm over several plans comes from one
+    ``GradNormPlan`` as their ``total_norm``.  Returns the gradient norm before the clip where it is needed (max_norm or skip_nonfinite; a 0-d
     fp32 tensor that the next run overwrites, or the ``total_norm`` given), else None."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], weights: Sequence | None = None,

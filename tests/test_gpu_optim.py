@@ -473,6 +473,72 @@ def test_adamw_any_dense_layout_and_fresh_moments(cuda):
         torch.testing.assert_close(x, o - 0.01 * y.sign(), rtol=0, atol=1e-6)
 
 
+# ---- random lists ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seed", range(24))
+def test_random_lists(cuda, seed):
+    """Lists of random lengths, sizes (around the pieces too), types and starts through all forms, in one packed buffer per role as
+    trainers hold them; what lies between the tensors stays."""
+    import random
+
+    rng = random.Random(1000 + seed)
+    n = rng.choice([1, 2, 7, 40, 200])
+    base = [1, 3, 255, 1023, 4096, 8192, ITEM, 2 * ITEM]
+    sizes = [max(0, rng.choice(base) * rng.choice([1, 1, 2]) + rng.randint(-3, 3)) if rng.random() < 0.7 else rng.randint(0, 40000) for _ in range(n)]
+    norm_type = rng.choice([2.0, 2.0, math.inf])
+
+    def packed(dtype, scale):
+        gaps = [rng.choice([0, 0, 1, 2, 7, 64]) for _ in range(n + 1)]
+        total = sum(sizes) + sum(gaps)
+        buf = torch.full((total,), 7.0, dtype=dtype, device=cuda)
+        keep = torch.ones(total, dtype=torch.bool, device=cuda)
+        views, at = [], gaps[0]
+        for i, k in enumerate(sizes):
+            v = buf[at:at + k]
+            v.normal_().mul_(scale)
+            keep[at:at + k] = False
+            views.append(v)
+            at += k + gaps[i + 1]
+        return views, lambda: bool((buf[keep] == 7).all())
+
+    gd, od, wd = rng.choice([BF16, F16, F32]), rng.choice([BF16, F16, F32]), rng.choice([None, BF16, F16])
+    (g, g_ok), (o, o_ok) = packed(gd, 0.05), packed(od, 1.0)
+    ref = norm_of(g, norm_type)
+    check_norm(slime_amd.get_total_norm(g, norm_type), g, norm_type)
+    total, each = slime_amd.GradNormPlan(g, norm_type, per_tensor=True).run()
+    check_norm(total, g, norm_type)
+    for e, t in zip(each, g):
+        check_norm(e, [t], norm_type)
+    before = [t.clone() for t in g]
+    max_norm, scale = ref * rng.choice([0.3, 0.9, 2.0]) + 1e-3, rng.choice([1.0, 0.5, 0.01])
+    slime_amd.GradClipPlan(g, norm_type, out=o).run(max_norm * scale, grad_scale=scale)
+    check_clip(o, before, max_norm * scale, ref * scale, scale)
+    assert all(torch.equal(a, b) for a, b in zip(g, before))
+    if rng.random() < 0.5:
+        slime_amd.GradClipPlan(g, norm_type).run(max_norm)
+    else:
+        ps = [torch.nn.Parameter(torch.empty_like(t)) for t in g]
+        for p, t in zip(ps, g):
+            p.grad = t
+        slime_amd.clip_grad_norm_(ps, max_norm, norm_type)
+    check_clip(g, before, max_norm, ref)
+    (p, p_ok), (m, m_ok), (v, v_ok) = packed(F32, 0.05), packed(F32, 0.02), packed(F32, 0.02)
+    w, w_ok = packed(wd, 1.0) if wd else ([None] * n, lambda: True)
+    for x in v:
+        x.square_()
+    old, ref = [[x.clone() for x in xs] for xs in (p, m, v)], norm_of(g, norm_type)
+    clip = rng.random() < 0.7
+    plan = slime_amd.AdamWPlan(p, g, w, m, v, betas=(0.8, 0.99), eps=1e-6, weight_decay=0.2, norm_type=norm_type, step=3)
+    plan.run(1e-2, max_norm=max_norm * scale if clip else None, grad_scale=scale)
+    c = scale * (min(1.0, max_norm * scale / (ref * scale + 1e-6)) if clip else 1.0)
+    for i in range(n):
+        want = adamw_bounds(g[i], old[0][i], old[1][i], old[2][i], 4, c, 1e-2, 1.0, 0.2, 0.8, 0.99, 1e-6, 5)
+        for x, (val, bound) in zip((p[i], m[i], v[i]), want):
+            near(x, val, bound)
+        if wd:
+            assert torch.equal(w[i], p[i].to(wd))
+    assert all(ok() for ok in (g_ok, o_ok, p_ok, m_ok, v_ok, w_ok))
+
+
 # ---- streams, graphs, and the run of them together ------------------------------------------------------------------------
 def test_plans_run_on_another_stream(cuda):
     ts = tensors([(1000, 999)] * 3, [BF16], 50)
