@@ -16,13 +16,14 @@ namespace wq {
 
 // One wavefront per workgroup and one 16-byte access per lane and stream (256 elements), 12 of them on a CU by an unused
 // dynamic LDS allocation: eight streams at once want few bytes in flight and short-lived workgroups.  604 M elements with
-// fp32 gradients, norm (320 us) included: 3150 us, 6.4 TB/s in the update, where the best of 1800 shapes of a bare kernel
+// fp32 gradients, norm (330 us) included: 3150-3190 us, 6.4 TB/s in the update, where the best of 1800 shapes of a bare kernel
 // without any table got 6.43; 256 threads on 2048 elements and 3 workgroups per CU 3290, on 1024 and 4 3380, on 2048 and 8
-// 3600 us; `nt` instead of `nt sc1` stores 3250 us.  807 M elements with bf16 gradients: 3760 us (219 of norm).
+// 3600 us; `nt` instead of `nt sc1` stores 3250 us; 15 wavefronts on a CU 3300 us.  Runs of 512 parts per XCD rather than 256: the
+// same at this size, 326 for 334 us on 75 M elements.  807 M elements with bf16 gradients: 3770 us (219 of norm).
 constexpr int kAdamThreads = 64;
 constexpr int kAdamPart = 256;                        // elements of a workgroup
 constexpr int kAdamParts = kAdamItem / kAdamPart;
-constexpr int kAdamPartsPerXcdRun = 256;
+constexpr int kAdamPartsPerXcdRun = 512;
 constexpr unsigned kAdamOccupancyPadBytes = 13000;
 
 struct AdamControl {       // at the start of the workspace, written anew by every step
