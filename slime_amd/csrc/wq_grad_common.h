@@ -217,7 +217,7 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm, fl
 }
 
 // workspace: 64 bytes of AdamW's per-step values, one partial per piece, and the sums of kFoldGroup partials each that long
-// lists fold first: one workgroup folds up to kFoldDirect partials in 4-5 us, and a whole model's 900 000 are 870 per thread.
+// lists fold first (norms of 12 300 pieces 33.9 us in one fold, 35.8 in two; of 27 600 68.5 and 68.9; of 55 300 130.4 and 127.9).
 constexpr int64_t kGradControlBytes = 64;
 constexpr int64_t kFoldGroup = 4096, kFoldDirect = 4 * kFoldGroup;
 inline char* partials_of(void* workspace) { return (char*)workspace + kGradControlBytes; }
