@@ -19,6 +19,7 @@ from __future__ import annotations
 import math
 import numbers
 from array import array
+from bisect import bisect_left
 from contextlib import nullcontext
 from typing import Iterable, Sequence
 
@@ -207,6 +208,11 @@ class _Plan:
     events): they share the workspace and the result.  The stream need not be the one the plan was built on.  The plan reads
     and writes the tensors it was given, wherever their contents come from; one that moves needs a new plan."""
 
+    # Tensors that a run writes while others of its workgroups may still read the run's device scalars (an AdamW run has read its
+    # scalars before it writes any).
+    _written_beside_reads: Sequence[torch.Tensor] = ()
+    _spans = None
+
     def _build(self, rows, device, what: str) -> None:
         self.device, self._what = device, what
         with torch.cuda.device(device):
@@ -230,10 +236,24 @@ class _Plan:
         factor, address = _scale_args(value, self.device, f"{self._what}: {what}")
         if address is not None and address == self.total_norm.data_ptr():
             raise ValueError(f"{self._what}: {what} must not be the plan's own total_norm, which the run overwrites")
+        self._refuse_written(address, what)
         return factor, address
 
     def _given(self, total_norm):
-        return None if total_norm is None else _scalar_on_device(total_norm, self.device, f"{self._what}: total_norm")
+        address = None if total_norm is None else _scalar_on_device(total_norm, self.device, f"{self._what}: total_norm")
+        self._refuse_written(address, "total_norm")
+        return address
+
+    def _refuse_written(self, address, what: str) -> None:
+        if address is None or not self._written_beside_reads:
+            return
+        if self._spans is None:             # they share no memory, so their starts and their ends have one order
+            spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in self._written_beside_reads if t.numel())
+            self._spans = [s for s, _ in spans], [e for _, e in spans]
+        starts, ends = self._spans
+        i = bisect_left(starts, address + 4) - 1
+        if i >= 0 and address < ends[i]:
+            raise ValueError(f"{self._what}: {what} must not lie in a tensor that the run writes")
 
 
 def _check_grads(grads, what: str):
@@ -253,7 +273,8 @@ class GradNormPlan(_Plan):
 
     ``run(grad_scale=1.0)`` returns ``total_norm``, a 0-d fp32 tensor that the next run overwrites, or ``(total_norm, norms)``
     with ``norms`` fp32 ``[len(grads)]``.  grad_scale (a number or one fp32 value on the device: an inverse loss scale, one over
-    the number of tokens) multiplies the gradients.  A gradient may be in the list twice and then counts twice."""
+    the number of tokens; not a value that the run writes) multiplies the gradients.  A gradient may be in the list twice and then
+    counts twice."""
 
     def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_tensor: bool = False):
         self._norm = _norm_selector(norm_type, "GradNormPlan")
@@ -262,6 +283,7 @@ class GradNormPlan(_Plan):
         self.norms = torch.zeros(len(self.grads), dtype=torch.float32, device=self.device) if per_tensor else None
         if per_tensor:
             self._owned.append(self.norms)
+            self._written_beside_reads = [self.norms]
         self._built()
 
     def run(self, grad_scale=1.0):
@@ -280,7 +302,7 @@ class GradClipPlan(_Plan):
 
     ``run(max_norm, grad_scale=1.0, total_norm=None)`` returns the norm before the clip: a 0-d fp32 tensor that the next run
     overwrites.  ``total_norm`` (one fp32 value on the device, of the gradients times grad_scale) is taken for the norm, and
-    returned, if it is given."""
+    returned, if it is given.  Device scalars must not lie in the tensors that are written."""
 
     def __init__(self, grads: Sequence[torch.Tensor], norm_type: float = 2.0, out: Sequence[torch.Tensor] | None = None):
         self._norm = _norm_selector(norm_type, "GradClipPlan")
@@ -296,6 +318,7 @@ class GradClipPlan(_Plan):
         apart = [g for g, o in zip(self.grads, self.out) if g is not o and (g.data_ptr() != o.data_ptr() or g.dtype != o.dtype)]
         _refuse_overlaps(self.out, apart, "GradClipPlan")
         self._build(_grad_rows(self.grads, self.out), _one_device(self.grads + self.out, "GradClipPlan"), "GradClipPlan")
+        self._written_beside_reads = self.out
         self._built()
 
     def run(self, max_norm: float, grad_scale=1.0, total_norm: torch.Tensor | None = None) -> torch.Tensor:

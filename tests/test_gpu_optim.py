@@ -753,3 +753,30 @@ def test_a_list_of_more_than_four_gigabytes(cuda):
 
 def test_abi_constants_match(cuda):
     assert _lib.GRAD_ITEM_BYTES == ITEM and 2 * _lib.ADAMW_ITEM == ITEM
+
+
+# ---- device scalars that lie in tensors of the call -----------------------------------------------------------------------
+def test_scalars_inside_tensors_of_a_plan(cuda):
+    """A scale among the gradients that a plan only reads is an ordinary value; one that its run writes is refused; an AdamW run
+    has read its scalars before it writes."""
+    g = tensors([(3 * ITEM + 5,), (4,), (300, 520)], [F32], 100, 0.2)
+    g[1][2] = 0.37
+    plan = slime_amd.GradNormPlan(g, per_tensor=True)
+    total, each = plan.run(grad_scale=g[1][2])
+    check_norm(total, g, scale=g[1][2].item())
+    for bad in plan.norms:
+        with pytest.raises(ValueError, match="must not lie in"):
+            plan.run(grad_scale=bad)
+    clip = slime_amd.GradClipPlan(g)
+    with pytest.raises(ValueError, match="must not lie in"):
+        clip.run(1.0, grad_scale=g[1][2])
+    with pytest.raises(ValueError, match="must not lie in"):
+        clip.run(1.0, total_norm=g[0][5])
+    a, b = (adamw_case([(2 * ITEM + 1,), (5,)], [BF16], [BF16], 101) for _ in range(2))
+    for x in (a, b):
+        x[0][1][3], x[0][1][4] = 2.0 ** -9, 0.125
+    pa, pb = (slime_amd.AdamWPlan(x[0], x[3], x[4], x[1], x[2]) for x in (a, b))
+    pa.run(2.0 ** -9, max_norm=0.5, grad_scale=0.125)
+    pb.run(b[0][1][3], max_norm=0.5, grad_scale=b[0][1][4])
+    for xs, ys in zip(a[:3] + (a[4],), b[:3] + (b[4],)):
+        assert all(torch.equal(x, y) for x, y in zip(xs, ys))

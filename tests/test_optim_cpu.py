@@ -373,3 +373,54 @@ def test_list_overlaps():
         for more in (buf[:1], buf[count * 10 - 1:], ts[count // 2], buf):
             with pytest.raises(ValueError, match="share memory"):
                 check(ts + [more])
+
+
+# ---- device scalars --------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def host_plans(monkeypatch):
+    """Plans over host tensors: everything but the tables, the workspace and the launches; -> the launches that were asked for."""
+    calls = []
+
+    def build(self, rows, device, what):
+        self.device, self._what = device, what
+        self.total_norm = torch.zeros((), dtype=torch.float32)
+        self._owned, self._n_items = [self.total_norm], 1
+        self._items = self._starts = self._workspace = self.total_norm
+
+    monkeypatch.setattr(optim, "_one_device", lambda tensors, what: torch.device("cpu"))
+    monkeypatch.setattr(optim._Plan, "_build", build)
+    monkeypatch.setattr(optim._Plan, "_built", lambda self: None)
+    monkeypatch.setattr(optim._Plan, "_run", lambda self, *args: calls.append(args))
+    return calls
+
+
+def test_plans_refuse_scalars_in_what_they_write(host_plans):
+    """The norm of tensor i is written by its workgroup while the others read the scale: a scale there is a race."""
+    g = _lists(4)
+    plan = optim.GradNormPlan(g, per_tensor=True)
+    for scale in (plan.norms[0], plan.norms[3], plan.norms[1:2]):
+        with pytest.raises(ValueError, match="grad_scale must not lie in"):
+            plan.run(grad_scale=scale)
+    with pytest.raises(ValueError, match="own total_norm"):
+        plan.run(grad_scale=plan.total_norm)
+    plan.run(grad_scale=g[0][0, 0])                                       # gradients are only read here
+    assert len(host_plans) == 1
+    buf = torch.zeros(100)
+    half = torch.zeros(20, dtype=torch.bfloat16)
+    plan = optim.GradClipPlan([buf[10:20], buf[30:30], buf[40:41], half[:3]])
+    odd = half.view(torch.float32)[1:2]                                   # its first half is written
+    for bad in (buf[10], buf[19], buf[40:41], odd):
+        with pytest.raises(ValueError, match="grad_scale must not lie in"):
+            plan.run(1.0, grad_scale=bad)
+        with pytest.raises(ValueError, match="total_norm must not lie in"):
+            plan.run(1.0, total_norm=bad)
+    for good in (buf[9], buf[20], buf[30], buf[39], buf[41], half.view(torch.float32)[2]):
+        plan.run(1.0, grad_scale=good, total_norm=good)
+    plan.run(1.0, total_norm=plan.total_norm)                             # not written when a norm is given
+    apart = optim.GradClipPlan([buf[0:4]], out=[buf[50:54]])
+    apart.run(1.0, grad_scale=buf[0], total_norm=buf[3])
+    with pytest.raises(ValueError, match="must not lie in"):
+        apart.run(1.0, total_norm=buf[53])
+    # an AdamW run has read its scalars before it writes
+    adamw = optim.AdamWPlan([buf[60:64]], [buf[70:74]])
+    adamw.run(buf[60], grad_scale=buf[70], total_norm=buf[61])
