@@ -132,6 +132,12 @@ def _refuse_overlaps(written, read, what: str) -> None:
         raise ValueError(f"{what}: tensors that are written share memory with others of the call (the same tensor twice?)")
 
 
+def _lies_in(address: int, starts, ends) -> bool:
+    """Whether an fp32 value at the address shares a byte with one of the ranges (disjoint, ascending)."""
+    i = bisect_left(starts, address + 4) - 1
+    return i >= 0 and address < ends[i]
+
+
 def _scalar_on_device(value, device, what: str):
     if value.dtype != torch.float32 or value.numel() != 1 or value.device != device:
         raise ValueError(f"{what} must be a number or one float32 value on {device}")
@@ -247,12 +253,10 @@ class _Plan:
     def _refuse_written(self, address, what: str) -> None:
         if address is None or not self._written_beside_reads:
             return
-        if self._spans is None:             # they share no memory, so their starts and their ends have one order
+        if self._spans is None:             # they share no memory
             spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in self._written_beside_reads if t.numel())
             self._spans = [s for s, _ in spans], [e for _, e in spans]
-        starts, ends = self._spans
-        i = bisect_left(starts, address + 4) - 1
-        if i >= 0 and address < ends[i]:
+        if _lies_in(address, *self._spans):
             raise ValueError(f"{self._what}: {what} must not lie in a tensor that the run writes")
 
 
@@ -477,7 +481,8 @@ class _List:
     def _refuse_overlaps(self, what: str) -> None:
         if len(self.ptr) <= 16:             # the arrays below cost 8 us however short they are
             spans = sorted((p, p + n * (4 if d == _lib.DTYPE_F32 else 2)) for p, n, d in zip(self.ptr, self.n, self.dtype) if n)
-            overlap = any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+            start, end = [s for s, _ in spans], [e for _, e in spans]
+            overlap = any(map(int.__lt__, start[1:], end))
         else:
             at, n = np.frombuffer(self.ptr, np.int64), np.frombuffer(self.n, np.int64)
             order = np.argsort(at[n > 0], kind="stable")
@@ -486,6 +491,11 @@ class _List:
             overlap = (start[1:] < end[:-1]).any()
         if overlap:
             raise ValueError(f"{what}: gradients share memory (the same tensor twice?); they cannot be clipped in place")
+        self.spans = start, end
+
+    def writes(self, address: int) -> bool:
+        """Whether the fp32 value there lies in a tensor of the list."""
+        return _lies_in(address, *self.spans)
 
     def workspace(self) -> torch.Tensor:
         """Kept by the caller until the launches are out; what comes after them on the stream may reuse it.  Large enough for
@@ -529,6 +539,8 @@ def _clip(grads: _List, max_norm: float, norm: int, total_norm, what: str) -> to
         _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, None, workspace.data_ptr(), total.data_ptr())
     else:
         total = total_norm.detach().to(device=device, dtype=torch.float32)
+        if grads.writes(total.data_ptr()):  # one workgroup would scale it while others read it
+            total = total.clone()
         _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, total.data_ptr(), None, None)
     _bump(grads.tensors)
     with torch.no_grad() if grads.copies else nullcontext():

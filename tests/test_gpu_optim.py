@@ -780,3 +780,17 @@ def test_scalars_inside_tensors_of_a_plan(cuda):
     pb.run(b[0][1][3], max_norm=0.5, grad_scale=b[0][1][4])
     for xs, ys in zip(a[:3] + (a[4],), b[:3] + (b[4],)):
         assert all(torch.equal(x, y) for x, y in zip(xs, ys))
+
+
+@pytest.mark.parametrize("n", [1, 3, 200])
+def test_clip_by_a_norm_that_is_among_the_gradients(cuda, n):
+    """The norm as it is at the call, as torch has it, in all launches of a long list."""
+    ts = tensors([(3 * ITEM + 5,)] + [(5,)] * (n - 1), [F32], 102)
+    ts[0][7] = 50.0
+    before = [t.clone() for t in ts]
+    ps = [torch.nn.Parameter(torch.empty_like(t)) for t in ts]
+    for p, t in zip(ps, ts):
+        p.grad = t
+    slime_amd.clip_grads_with_norm_(ps, 2.0, ts[0][7])
+    check_clip(ts, before, 2.0, 50.0)
+    check_guards(ts)

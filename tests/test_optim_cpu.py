@@ -424,3 +424,28 @@ def test_plans_refuse_scalars_in_what_they_write(host_plans):
     # an AdamW run has read its scalars before it writes
     adamw = optim.AdamWPlan([buf[60:64]], [buf[70:74]])
     adamw.run(buf[60], grad_scale=buf[70], total_norm=buf[61])
+
+
+def _host_list(monkeypatch):
+    """Lists over host tensors, and -> what the launches were given."""
+    calls = []
+    to = torch.Tensor.to
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *a, device=None, **k: to(t, *a, **k))
+    monkeypatch.setattr(optim, "_one_device", lambda tensors, what: torch.device("cuda", 0))
+    monkeypatch.setattr(optim, "_launch", lambda device, entry, what, *args: calls.append((entry, args)))
+    monkeypatch.setattr(optim._List, "workspace", lambda self: torch.empty(64, dtype=torch.int64))
+    return calls
+
+
+@pytest.mark.parametrize("count", [3, 40])
+def test_a_given_norm_among_the_gradients_is_copied_first(monkeypatch, count):
+    """Scaled in place by one workgroup (or by an earlier launch of a long list) while others read it as the norm."""
+    calls = _host_list(monkeypatch)
+    buf = torch.arange(10.0 * count + 10)
+    ps = _params([buf[10 * i:10 * i + 9] for i in range(count)])
+    for k in (0, 4, 8, 10 * count - 2):
+        slime_amd.clip_grads_with_norm_(ps, 1.0, buf[k])
+        assert calls[-1][0] == "wq_grad_clip_list" and calls[-1][1][-3] != buf[k].data_ptr()
+    for k in (9, 19, 10 * count - 1, 10 * count):
+        slime_amd.clip_grads_with_norm_(ps, 1.0, buf[k])
+        assert calls[-1][1][-3] == buf[k].data_ptr()
