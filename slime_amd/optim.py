@@ -138,16 +138,18 @@ def _lies_in(address: int, starts, ends) -> bool:
     return i >= 0 and address < ends[i]
 
 
-def _scalar_on_device(value, device, what: str):
-    if value.dtype != torch.float32 or value.numel() != 1 or value.device != device:
-        raise ValueError(f"{what} must be a number or one float32 value on {device}")
-    return value.data_ptr()
+def _scalar_on_device(value, device, what: str, number: str = "") -> int:
+    """The address of a scalar argument; a sharded or wrapped tensor has none (0, which the kernels take for "not given")."""
+    if not isinstance(value, torch.Tensor) or value.dtype != torch.float32 or value.numel() != 1 or value.device != device or \
+            value.layout != torch.strided or value.is_neg() or not (address := value.data_ptr()):
+        raise ValueError(f"{what} must be {number}one float32 value on {device} (of a sharded tensor, the full one)")
+    return address
 
 
 def _scale_args(scale, device, what: str):
     """-> (factor, address of a factor on the device or None)"""
     if isinstance(scale, torch.Tensor):
-        return 1.0, _scalar_on_device(scale, device, what)
+        return 1.0, _scalar_on_device(scale, device, what, "a number or ")
     scale = float(scale)
     if not 0.0 <= scale < math.inf:
         raise ValueError(f"{what} must be a finite number that is not negative, got {scale}")
@@ -538,7 +540,7 @@ def _clip(grads: _List, max_norm: float, norm: int, total_norm, what: str) -> to
         total, workspace = torch.empty((), dtype=torch.float32, device=device), grads.workspace()
         _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, None, workspace.data_ptr(), total.data_ptr())
     else:
-        total = total_norm.detach().to(device=device, dtype=torch.float32)
+        total = total_norm.detach().resolve_neg().to(device=device, dtype=torch.float32)
         if grads.writes(total.data_ptr()):  # one workgroup would scale it while others read it
             total = total.clone()
         _launch(device, "wq_grad_clip_list", what, *grads.args, norm, max_norm, 1.0, total.data_ptr(), None, None)
@@ -571,6 +573,8 @@ def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max
     max_norm = _check_max_norm(max_norm, "clip_grads_with_norm_")
     if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1:
         raise TypeError("clip_grads_with_norm_: total_norm must be a tensor of one value")
+    if hasattr(total_norm, "to_local"):
+        raise TypeError("clip_grads_with_norm_: total_norm must be a plain tensor (of a sharded one, pass the full tensor)")
     grads = _grads_of(parameters)
     if grads:
         what = "clip_grads_with_norm_"

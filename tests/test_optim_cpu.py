@@ -449,3 +449,35 @@ def test_a_given_norm_among_the_gradients_is_copied_first(monkeypatch, count):
     for k in (9, 19, 10 * count - 1, 10 * count):
         slime_amd.clip_grads_with_norm_(ps, 1.0, buf[k])
         assert calls[-1][1][-3] == buf[k].data_ptr()
+
+
+def test_scalars_without_an_address_are_refused(host_plans):
+    """A wrapper (a sharded tensor, say) has address 0, which the kernels take for "not given": the norm of the local part, a scale
+    or a learning rate of one."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls):
+            return torch.Tensor._make_wrapper_subclass(cls, (), dtype=torch.float32, device="cpu")
+
+        def to_local(self):
+            return None
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError
+
+    wrapped, flipped = Wrapper(), torch._neg_view(torch.ones(()))
+    assert wrapped.data_ptr() == 0
+    norm, clip, adamw = optim.GradNormPlan(_lists()), optim.GradClipPlan(_lists()), optim.AdamWPlan(_lists(), _lists())
+    for bad in (wrapped, flipped, torch.ones(1).to_sparse()):
+        for call in (lambda: norm.run(grad_scale=bad), lambda: clip.run(1.0, grad_scale=bad), lambda: clip.run(1.0, total_norm=bad),
+                     lambda: adamw.run(bad), lambda: adamw.run(1.0, grad_scale=bad), lambda: adamw.run(1.0, 1.0, total_norm=bad)):
+            with pytest.raises(ValueError, match="one float32 value"):
+                call()
+    for call in (lambda: clip.run(1.0, total_norm=2.0), lambda: adamw.run(1.0, 1.0, total_norm=2.0)):
+        with pytest.raises(ValueError, match="total_norm must be one float32 value"):
+            call()
+    with pytest.raises(TypeError, match="full tensor"):
+        slime_amd.clip_grads_with_norm_(_params(_lists()), 1.0, wrapped)
+    assert not host_plans
+    clip.run(1.0, grad_scale=torch.nn.Parameter(torch.ones(1)), total_norm=torch.ones(1, 1))
