@@ -193,6 +193,11 @@ def _cuts(rows: np.ndarray):
     return _lib.GRAD_ITEM_BYTES // g, np.where((rows[:, 1] != 0) & (o >= g), rows[:, 1] % 128 // o, rows[:, 0] % 128 // g)
 
 
+def _refuse_no_memory(addresses: np.ndarray, what: str) -> None:
+    if (addresses == 0).any():
+        raise ValueError(f"{what}: a tensor has no memory (a wrapper, or storage that was released)")
+
+
 def _item_table(rows: np.ndarray, device, what: str):
     """Per-tensor rows (int64 [n, 4 or 8], the fields of wq_grad_desc / wq_adamw_desc) -> (item table on the device, starts
     of the tensors in it, number of items)."""
@@ -200,6 +205,7 @@ def _item_table(rows: np.ndarray, device, what: str):
     g, out = (np.where(d == _lib.DTYPE_F32, 4, 2) for d in (rows[:, 3] & 0xFFFFFFFF, rows[:, 3] >> 32))
     if (rows[:, 0] % g).any() or (rows[:, 1] % out).any() or (rows[:, 4:7] % 4).any():
         raise ValueError(f"{what}: a tensor does not start at a multiple of its element size")
+    _refuse_no_memory(rows[n > 0][:, [0, 4, 5, 6] if rows.shape[1] == 8 else [0, 1]], what)
     starts = np.zeros(len(rows) + 1, dtype=np.int64)
     per, phase = _cuts(rows)
     np.cumsum(np.where(n > 0, -(-(n + phase) // per), 0), out=starts[1:])
@@ -407,6 +413,7 @@ class AdamWPlan(_Plan):
         has = np.array([w is not None for w in self.weights])
         rows[:, 1], rows[:, 3] = 0, rows[:, 3] & 0xFFFFFFFF
         rows[has, 1] = _column(_data_ptr, [w for w in self.weights if w is not None])
+        _refuse_no_memory(rows[has & (rows[:, 2] > 0), 1], "AdamWPlan")      # further on a 0 stands for "no copy"
         rows[has, 3] |= _column(_DTYPES.get, [w.dtype for w in self.weights if w is not None]) << 32
         for k, xs in enumerate((self.params, self.exp_avgs, self.exp_avg_sqs)):
             rows[:, 4 + k] = _column(_data_ptr, xs)

@@ -481,3 +481,20 @@ def test_scalars_without_an_address_are_refused(host_plans):
         slime_amd.clip_grads_with_norm_(_params(_lists()), 1.0, wrapped)
     assert not host_plans
     clip.run(1.0, grad_scale=torch.nn.Parameter(torch.ones(1)), total_norm=torch.ones(1, 1))
+
+
+def test_tensors_without_memory_are_refused(host_plans):
+    """Released storage and wrappers have address 0; the table would send the kernels there."""
+    F = _lib.DTYPE_F32
+    released = torch.zeros(8)
+    released.untyped_storage().resize_(0)
+    for row in ([released.data_ptr(), 1024, 8, F], [1024, 0, 8, F], [0, 0, 8, F, 1024, 1024, 1024, 0], [1024, 0, 8, F, 0, 1024, 1024, 0],
+                [1024, 0, 8, F, 1024, 0, 1024, 0], [1024, 0, 8, F, 1024, 1024, 0, 0]):
+        empty = [1024, 1024, 0, F] if len(row) == 4 else [0, 0, 0, F, 0, 0, 0, 0]
+        with pytest.raises(ValueError, match="no memory"):
+            optim._item_table(np.array([empty, row], dtype=np.int64), torch.device("cpu"), "x")
+    weight = torch.zeros(4, 8, dtype=torch.bfloat16)
+    weight.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="no memory"):                    # it would not be written
+        optim.AdamWPlan(_lists(1), _lists(1), weights=[weight])
+    optim.AdamWPlan(_lists(1, shape=(0, 3)), _lists(1, shape=(0, 3)), weights=_lists(1, torch.bfloat16, (0, 3)))
