@@ -95,6 +95,38 @@ def _check_no_self_overlap(t, what: str) -> None:
         reach += st * (n - 1)
 
 
+class _Elements:
+    """What numpy needs to know of a tensor's elements to tell whether they share memory with others'; it follows no address."""
+
+    def __init__(self, t):
+        size = t.element_size()
+        self.__array_interface__ = {"version": 3, "data": (t.data_ptr(), False), "shape": tuple(t.shape), "typestr": f"|V{size}",
+                                    "strides": tuple(st * size for st in t.stride())}
+
+
+def _share_memory(tensors) -> bool:
+    """Whether two of the tensors share an element, exactly: slices that interleave do not.  Tensors whose byte ranges meet are
+    compared in pairs (1.5 us each); the few pairs of strides that would take numpy milliseconds count as sharing."""
+    spans = sorted(((t.data_ptr(), t.data_ptr() + (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))) * t.element_size(), i)
+                    for i, t in enumerate(tensors) if t.numel()))
+    arrays, open_ = {}, []
+    for start, end, i in spans:
+        open_ = [(e, j) for e, j in open_ if e > start]
+        for _, j in open_:
+            if _is_dense(tensors[i]) and _is_dense(tensors[j]):
+                return True
+            for k in (i, j):
+                if k not in arrays:
+                    arrays[k] = np.asarray(_Elements(tensors[k]))
+            try:
+                if np.shares_memory(arrays[i], arrays[j], max_work=100_000):
+                    return True
+            except np.exceptions.TooHardError:
+                return True
+        open_.append((end, i))
+    return False
+
+
 def _same_layout(a, b) -> bool:
     return a.shape == b.shape and (a.stride() == b.stride() or a.numel() == 0 or
                                    all(n == 1 or x == y for x, y, n in zip(a.stride(), b.stride(), a.shape)))
@@ -447,13 +479,16 @@ def _grads_of(parameters) -> list:
     return [g for p in parameters if (g := p.grad) is not None]
 
 
+_SHARED = "gradients share memory (the same tensor twice?); they cannot be clipped in place"
+
+
 class _List:
     """Tensors as the list entry points take them: host arrays of addresses, element counts and types.  The common case -
     contiguous tensors of one GPU - is found out by passes that stay in C (0.2 us a tensor); anything else is looked at
     one by one, for the message or for the copies that other strides need."""
 
     def __init__(self, tensors, what: str, written: bool):
-        self.copies = []
+        self.copies, given = [], tensors
         selectors = None
         if set(map(type, tensors)) <= _PLAIN_TYPES:
             try:
@@ -470,6 +505,8 @@ class _List:
         self.dtype = array("i", selectors)
         if written:
             self._refuse_overlaps(what)
+            if self.copies and _share_memory(given):      # of the originals: the copies lie apart
+                raise ValueError(f"{what}: {_SHARED}")
         self.args = (self.ptr.buffer_info()[0], self.n.buffer_info()[0], self.dtype.buffer_info()[0], len(tensors))
 
     def _one_by_one(self, tensors, what: str, written: bool):
@@ -499,7 +536,7 @@ class _List:
             end = start + (n * np.where(np.frombuffer(self.dtype, np.int32) == _lib.DTYPE_F32, 4, 2))[n > 0][order]
             overlap = (start[1:] < end[:-1]).any()
         if overlap:
-            raise ValueError(f"{what}: gradients share memory (the same tensor twice?); they cannot be clipped in place")
+            raise ValueError(f"{what}: {_SHARED}")
         self.spans = start, end
 
     def writes(self, address: int) -> bool:

@@ -498,3 +498,60 @@ def test_tensors_without_memory_are_refused(host_plans):
     with pytest.raises(ValueError, match="no memory"):                    # it would not be written
         optim.AdamWPlan(_lists(1), _lists(1), weights=[weight])
     optim.AdamWPlan(_lists(1, shape=(0, 3)), _lists(1, shape=(0, 3)), weights=_lists(1, torch.bfloat16, (0, 3)))
+
+
+@pytest.mark.parametrize("clip", [lambda ps: slime_amd.clip_grad_norm_(ps, 1.0),
+                                  lambda ps: slime_amd.clip_grads_with_norm_(ps, 1.0, torch.ones(()))])
+def test_strided_gradients_that_share_memory_are_refused(monkeypatch, clip):
+    """They are scaled by way of copies, which lie apart: their elements counted twice in the norm and were scaled once."""
+    calls = _host_list(monkeypatch)
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **k: empty(*a, **k))
+    x, h = torch.randn(6, 8, 10), torch.randn(6, 8, dtype=torch.float32).to(torch.bfloat16)
+    crossing = torch.zeros(200).as_strided((3, 4, 2), (50, 7, 3))
+    for shared in ([x[:, :3], x[:, :3]], [x, x[:, :3]], [x[:, :3], x], [x[0], x[..., ::2]], [x[:, :3], x[:, 2:5]],
+                   [x[..., ::2], x[..., 1::2], x[:, 3:4, 9:]], [x[:, :3].permute(2, 0, 1), x[2:3, 1:2, 4:5]],
+                   [h[:, ::2], h.view(torch.float32)[:, 1:3]], [crossing, torch.as_strided(crossing, (4, 5), (30, 2), 8)],
+                   [x[i, :, ::2] for i in range(6)] + [x[3, 4:6]]):
+        for order in (shared, shared[::-1]):
+            with pytest.raises(ValueError, match="share memory"):
+                clip(_params(order))
+    assert not calls
+    apart = [x[:, :3], x[:, 3:8, ::2], x[:, 3:8, 1::2].permute(1, 2, 0)]
+    for fine in (apart, apart[::-1], [x[:, :3], x[:, 3:3], x[:, 3:]], [x[..., ::3], x[..., 1::3], x[..., 2::3]], [h[:, ::2], h[:, 1::2]],
+                 [h[:, :2].T, h.view(torch.float32)[:, 1:3]], [x[i, :, j::4] for i in range(6) for j in range(4)],
+                 [x[1, 2, 3:5], x[1:, 3:], x[0]]):
+        before = [t.clone() for t in fine]
+        clip(_params(fine))
+        assert all(torch.equal(a, b) for a, b in zip(fine, before))      # nothing was launched: the copies come back as they were
+    assert calls
+    y = torch.zeros(64 * 9).view(9, 64)
+    assert not optim._share_memory([y[:, i] for i in range(64)])
+    assert optim._share_memory([y[:, i] for i in range(64)] + [y[4:5, 63:]])
+
+
+def test_shared_elements_against_a_count():
+    """Random pairs of strided views against the sets of their addresses."""
+    import random
+
+    rng = random.Random(5)
+    buf = torch.zeros(4000)
+    seen = set()
+
+    def view():
+        dims, reach, shape, stride = rng.randint(1, 3), 0, [], []
+        for _ in range(dims):
+            shape.append(rng.randint(1, 5))
+            stride.append(reach + rng.randint(1, 9))
+            reach += stride[-1] * (shape[-1] - 1)
+        order = rng.sample(range(dims), dims)
+        return buf.as_strided([shape[i] for i in order], [stride[i] for i in order], rng.randint(0, 60))
+
+    index = torch.arange(4000)
+    for _ in range(1500):
+        a, b = view(), view()
+        at = [set(index.as_strided(v.shape, v.stride(), v.storage_offset()).flatten().tolist()) for v in (a, b)]
+        shared = bool(at[0] & at[1])
+        assert optim._share_memory([a, b]) == shared
+        seen.add(shared)
+    assert seen == {True, False}
