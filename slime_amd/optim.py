@@ -104,17 +104,34 @@ class _Elements:
                                     "strides": tuple(st * size for st in t.stride())}
 
 
+def _run_and_pitch(t):
+    """-> (bytes of the runs of memory that the elements form, greatest common divisor of the distances between runs; 0 for one)"""
+    run, pitch, size = 1, 0, t.element_size()
+    for st, n in _strides(t):
+        if st == run and not pitch:
+            run *= n
+        else:
+            pitch = math.gcd(pitch, st)
+    return run * size, pitch * size
+
+
 def _share_memory(tensors) -> bool:
     """Whether two of the tensors share an element, exactly: slices that interleave do not.  Tensors whose byte ranges meet are
-    compared in pairs (1.5 us each); the few pairs of strides that would take numpy milliseconds count as sharing."""
-    spans = sorted(((t.data_ptr(), t.data_ptr() + (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))) * t.element_size(), i)
-                    for i, t in enumerate(tensors) if t.numel()))
-    arrays, open_ = {}, []
-    for start, end, i in spans:
-        open_ = [(e, j) for e, j in open_ if e > start]
-        for _, j in open_:
-            if _is_dense(tensors[i]) and _is_dense(tensors[j]):
+    compared in pairs, first by where their runs lie modulo the common pitch (0.4 us: slices of one buffer), then by numpy; the
+    few pairs of strides that would take that milliseconds count as sharing."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))) * t.element_size(),
+                    *_run_and_pitch(t), i) for i, t in enumerate(tensors) if t.numel())
+    arrays, meeting = {}, []
+    for span in spans:
+        start, _, run, pitch, i = span
+        meeting = [other for other in meeting if other[1] > start]
+        for from_, _, other_run, other_pitch, j in meeting:
+            common = math.gcd(pitch, other_pitch)
+            if not common:
                 return True
+            at = (start - from_) % common
+            if at >= other_run and at + run <= common:
+                continue
             for k in (i, j):
                 if k not in arrays:
                     arrays[k] = np.asarray(_Elements(tensors[k]))
@@ -123,7 +140,7 @@ def _share_memory(tensors) -> bool:
                     return True
             except np.exceptions.TooHardError:
                 return True
-        open_.append((end, i))
+        meeting.append(span)
     return False
 
 
