@@ -547,7 +547,7 @@ int wq_grad_clip_list(void *const *g, const int64_t *n, const int32_t *dtype, in
 /* One AdamW step (decoupled weight decay), all arithmetic in fp32 from fp32 state, t = step + 1, g' = coefficient * g:
  *   p1 = p - lr * lr_scale * weight_decay * p;  m = b1 * m + (1 - b1) * g';  v = b2 * v + (1 - b2) * g'^2
  *   p  = p1 - lr * lr_scale / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  out = round(p)
- * step: DEVICE int64, incremented by the call, so a recorded call counts its replays.  lr: host value, times lr_dev[0] if
+ * eps: 0 or a number that fp32 does not round to 0 (WQ_ERR_SHAPE).  step: DEVICE int64, incremented by the call, so a recorded call counts its replays.  lr: host value, times lr_dev[0] if
  * lr_dev is not NULL.  max_norm < 0: no clip (coefficient = grad_scale).  The norm is computed if it is needed (max_norm >= 0
  * or skip_nonfinite) and total_given is NULL.  skip_nonfinite: with an infinite or NaN norm nothing is written, `step`
  * included.  total: fp32, where a computed norm goes (NULL allowed if none is). */

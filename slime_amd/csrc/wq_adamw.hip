@@ -183,6 +183,7 @@ WQ_EXPORT int wq_adamw_items(const wq_adamw_desc* items, int64_t n_items, const 
     if (!h || !workspace || !h->step || (n_items && !items)) return WQ_ERR_NULL;
     if (h->norm != WQ_NORM_2 && h->norm != WQ_NORM_INF) return WQ_ERR_MODE;
     if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0)) return WQ_ERR_SHAPE;
+    if (h->eps > 0.0 && (float)h->eps == 0.0f) return WQ_ERR_SHAPE;   // 0 / 0 where the formula has 0
     const bool need_norm = h->max_norm >= 0.0f || h->skip_nonfinite;
     if (need_norm && !h->total_given && !h->total) return WQ_ERR_NULL;
     hipStream_t st = (hipStream_t)stream;

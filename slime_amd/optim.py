@@ -36,6 +36,7 @@ _NORMS = {2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 _data_ptr, _numel, _is_contiguous, _get_device, _is_neg = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device", "is_neg"))
 _dtype, _layout, _shape, _nbytes = (getattr(torch.Tensor, n).__get__ for n in ("dtype", "layout", "shape", "nbytes"))
 _PLAIN_TYPES = {torch.Tensor, torch.nn.Parameter}
+_F32_MAX = float(np.finfo(np.float32).max)      # what the kernels take as fp32 has to be finite there
 
 
 def _norm_selector(norm_type, what: str) -> int:
@@ -200,8 +201,8 @@ def _scale_args(scale, device, what: str):
     if isinstance(scale, torch.Tensor):
         return 1.0, _scalar_on_device(scale, device, what, "a number or ")
     scale = float(scale)
-    if not 0.0 <= scale < math.inf:
-        raise ValueError(f"{what} must be a finite number that is not negative, got {scale}")
+    if not 0.0 <= scale <= _F32_MAX:
+        raise ValueError(f"{what} must be a finite number (in fp32) that is not negative, got {scale}")
     return scale, None
 
 
@@ -396,8 +397,8 @@ def _per_tensor(value, n: int, what: str):
     if len(values) != n:
         raise ValueError(f"AdamWPlan: need one {what} per parameter")
     for v in values:
-        if not 0.0 <= v < math.inf:
-            raise ValueError(f"AdamWPlan: {what} must be finite and not negative, got {v}")
+        if not 0.0 <= v <= _F32_MAX:
+            raise ValueError(f"AdamWPlan: {what} must be finite (in fp32) and not negative, got {v}")
     return values
 
 
@@ -427,6 +428,8 @@ class AdamWPlan(_Plan):
         self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
         if not all(0.0 <= b < 1.0 for b in self.betas) or not 0.0 <= self.eps < math.inf:
             raise ValueError(f"AdamWPlan: betas must be in [0, 1) and eps finite and not negative, got {betas}, {eps}")
+        if 0.0 < self.eps <= 2.0 ** -150:       # 0 in fp32: elements without a gradient so far would become NaN
+            raise ValueError(f"AdamWPlan: eps must be 0 or above 2^-150, half of fp32's smallest number, got {eps}")
         if int(step) < 0:
             raise ValueError(f"AdamWPlan: step must not be negative, got {step}")
         self.grads, self.params = _check_grads(grads, "AdamWPlan"), list(params)

@@ -555,3 +555,23 @@ def test_shared_elements_against_a_count():
         assert optim._share_memory([a, b]) == shared
         seen.add(shared)
     assert seen == {True, False}
+
+
+def test_numbers_that_fp32_cannot_hold_are_refused(host_plans):
+    """Finite in 64 bits and infinite (or an eps of 0) in the kernels: every gradient or weight became infinite or NaN."""
+    clip, adamw = optim.GradClipPlan(_lists()), optim.AdamWPlan(_lists(), _lists())
+    most = float(np.finfo(np.float32).max)
+    for call in (lambda: clip.run(1.0, grad_scale=1e39), lambda: adamw.run(1e-3, grad_scale=3.5e38), lambda: adamw.run(1e39),
+                 lambda: optim.GradNormPlan(_lists()).run(1e300), lambda: optim.AdamWPlan(_lists(), _lists(), weight_decay=1e39),
+                 lambda: optim.AdamWPlan(_lists(), _lists(), lr_scale=[1.0, 1e39, 1.0])):
+        with pytest.raises(ValueError, match="finite .*in fp32"):
+            call()
+    for eps in (1e-50, 2.0 ** -150, 5e-324):
+        with pytest.raises(ValueError, match="eps"):
+            optim.AdamWPlan(_lists(), _lists(), eps=eps)
+        assert _lib.load().wq_adamw_items(P, 1, _hyper(eps=eps), P, None) == S
+    assert not host_plans
+    clip.run(1e39, grad_scale=most)                       # a limit above everything is no limit
+    optim.AdamWPlan(_lists(), _lists(), eps=1e-45).run(most)
+    optim.AdamWPlan(_lists(), _lists(), eps=0.0, weight_decay=most, lr_scale=most)
+    assert _lib.load().wq_adamw_items(None, 1, _hyper(eps=1e-45), P, None) == N_
