@@ -34,7 +34,7 @@ struct AdamControl {       // at the start of the workspace, written anew by eve
     int32_t skip;
     int32_t unused[3];
 };
-typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8), aligned(16)));     // a workspace has no more
 static_assert(sizeof(AdamControl) == sizeof(u32x8) && sizeof(AdamControl) <= kGradControlBytes, "workspace layout");
 
 struct AdamBeginArgs {

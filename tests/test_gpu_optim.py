@@ -794,3 +794,25 @@ def test_clip_by_a_norm_that_is_among_the_gradients(cuda, n):
     slime_amd.clip_grads_with_norm_(ps, 2.0, ts[0][7])
     check_clip(ts, before, 2.0, 50.0)
     check_guards(ts)
+
+
+# ---- the C entry points -----------------------------------------------------------------------------------------------------
+def test_workspaces_of_sixteen_byte_alignment(cuda):
+    """All entry points on a workspace that is aligned to 16 bytes and to no more."""
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    a, b = (adamw_case([(2 * ITEM + 1,), (5,)], [BF16], [BF16], 110) for _ in range(2))
+    plan = slime_amd.AdamWPlan(a[0], a[3], a[4], a[1], a[2])
+    plan.run(1e-2, max_norm=0.5, grad_scale=0.25)
+    other = slime_amd.AdamWPlan(b[0], b[3], b[4], b[1], b[2])
+    room = torch.zeros(lib.wq_grad_workspace_bytes(other._n_items) // 8 + 2, dtype=torch.int64, device=cuda)
+    h = other._hyper
+    h.lr, h.max_norm, h.grad_scale = 1e-2, 0.5, 0.25
+    assert room.data_ptr() % 32 == 0
+    assert lib.wq_adamw_items(other._items.data_ptr(), other._n_items, h, room.data_ptr() + 16, st) == 0
+    assert torch.equal(plan.total_norm, other.total_norm)
+    for xs, ys in zip(a[:3] + (a[4],), b[:3] + (b[4],)):
+        assert all(torch.equal(x, y) for x, y in zip(xs, ys))
+    total = torch.zeros((), device=cuda)
+    assert lib.wq_grad_norm_items(other._items.data_ptr(), other._n_items, 8, None, 0, 0, 0.25, None, room.data_ptr() + 16, total.data_ptr(),
+                                  None, st) == 0
+    assert torch.equal(total, plan.total_norm) and room[0].item() == 0 and room[1].item() == 0
