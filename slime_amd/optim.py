@@ -566,8 +566,7 @@ class _List:
     def workspace(self) -> torch.Tensor:
         """Kept by the caller until the launches are out; what comes after them on the stream may reuse it.  Large enough for
         any list of these sizes: as many pieces as fp32 has, and two more per tensor for where it starts."""
-        pieces = sum(self.n) * 4 // _lib.GRAD_ITEM_BYTES + 2 * len(self.n)
-        return torch.empty(8 + pieces + pieces // 4096 + 1, dtype=torch.int64, device=self.device)
+        return _workspace(sum(self.n) * 4 // _lib.GRAD_ITEM_BYTES + 2 * len(self.n), self.device)
 
 
 def _refuse_nonfinite(total: torch.Tensor, norm_type) -> None:
