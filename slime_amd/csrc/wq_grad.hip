@@ -3,8 +3,8 @@
 //   norm_2 = s * sqrt(sum g^2), norm_inf = s * max |g|, coefficient = s * min(1, max_norm / (norm + 1e-6)), out = round(g * c)
 //
 // Both are bound by HBM: the norm reads every gradient once, the clip reads it again and writes it.  One workgroup takes one
-// piece, 16 KiB of one tensor, and leaves one 64-bit partial; a fold of the partials in a fixed order
-// gives the norm (no atomics, so the same gradients give the same bits).  Squares are added in 64 bits: fp32 squares are
+// piece - 16 KiB of one tensor, in the table of an update the gradients of 8192 elements - and leaves one 64-bit partial; a fold of
+// the partials in a fixed order gives the norm (no atomics, so the same gradients give the same bits).  Squares are added in 64 bits: fp32 squares are
 // exact there and can neither overflow nor vanish.
 
 #include "wq_grad_common.h"
@@ -263,7 +263,14 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
 // A norm whose gradients are read again right away (`again`) leaves them in the 256 MB Infinity Cache if they fit: plain
 // instead of non-temporal loads make the norm alone slower (202 MB of bf16: 35 -> 38 us) and norm and clip together faster
 // (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 83 -> 80 us); with 2.4 GB nothing is left to find (1060 -> 1087 us).
+// The host knows the number of pieces only: a list of more small tensors than that is taken for a long one.
 constexpr int64_t kKeepPieces = (256 << 20) / WQ_GRAD_ITEM_BYTES;
+// The same for an update, whose pieces are 32 KiB of fp32 or 16 KiB of bf16 gradients and which comes back to a gradient while
+// it streams six arrays more; a part of a list beyond the cache is still found there.  With clip, non-temporal -> plain, fp32: 17 MB
+// 30.0 -> 28.3 us, 101 MB 139 -> 129, 252 MB 342 -> 313, 403 MB 536 -> 510, 604 MB 796 -> 775, 1.2 GB 1602 -> 1592, 1.8 GB 2394 ->
+// 2391, 4.8 GB 7230 -> 7279; bf16: 101 MB 242 -> 230, 252 MB 598 -> 569, 403 MB 949 -> 921, 0.8 GB 1907 -> 1890, 1.2 GB 2860 -> 2852,
+// 1.8 GB 4298 -> 4315.  32768 pieces are 1.1 GB of fp32 or 0.5 GB of bf16.
+constexpr int64_t kKeepAdamItems = 32768;
 
 template <int NORM, typename Source>
 static void launch_pieces(const Source& src, int64_t n_items, bool keep, char* partials, hipStream_t st)
@@ -291,15 +298,15 @@ static void launch_total(char* partials, int64_t n_items, float scale, const flo
     else grad_norm_total_kernel<NORM, 1024><<<1, 1024, 0, st>>>(p.at, p.n, scale, scale_dev, total);
 }
 template <int NORM>
-static Partials launch_table_partials(const TableSource& src, int64_t n_items, bool again, void* workspace, hipStream_t st)
+static Partials launch_update_partials(const TableSource& src, int64_t n_items, void* workspace, hipStream_t st)
 {
-    launch_pieces<NORM>(src, n_items, again && n_items <= kKeepPieces, partials_of(workspace), st);
+    launch_pieces<NORM>(src, n_items, n_items <= kKeepAdamItems, partials_of(workspace), st);
     return launch_fold<NORM>(partials_of(workspace), n_items, st);
 }
 Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st)
 {
-    return norm == WQ_NORM_2 ? launch_table_partials<WQ_NORM_2>(src, n_items, true, workspace, st)
-                             : launch_table_partials<WQ_NORM_INF>(src, n_items, true, workspace, st);
+    return norm == WQ_NORM_2 ? launch_update_partials<WQ_NORM_2>(src, n_items, workspace, st)
+                             : launch_update_partials<WQ_NORM_INF>(src, n_items, workspace, st);
 }
 template <int NORM>
 static void launch_table_norm(const TableSource& src, int64_t n_items, bool again, float scale, const float* scale_dev, void* workspace,

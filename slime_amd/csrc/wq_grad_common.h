@@ -226,8 +226,8 @@ struct Partials {
     int64_t n;
 };
 
-// wq_grad.hip: one partial per piece (of gradients that are read again right behind), for more than kFoldDirect pieces folded
-// to one value per kFoldGroup
+// wq_grad.hip: one partial per piece of an update's table (whose gradients are read again right behind), for more than
+// kFoldDirect pieces folded to one value per kFoldGroup
 Partials launch_norm_partials(const TableSource& src, int64_t n_items, int norm, void* workspace, hipStream_t st);
 
 }  // namespace wq
