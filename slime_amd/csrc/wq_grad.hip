@@ -195,8 +195,8 @@ __device__ __forceinline__ void piece_scale_from(const GradPiece& p, int part, f
 
 // NORM < 0: the norm is at `total`.  Otherwise every workgroup folds the list's partials for itself - kFoldByAll at most, a
 // microsecond - in the order in which the total's kernel would, and the first one writes the norm: a launch less where the
-// launches are most of the time (a clip of 65 pieces 20.0 -> 16.8 us, of 576 11.9 -> 9.1, of 1152 13.6 either way, of 2304
-// 20.0 -> 23.2 us: every workgroup's microsecond adds up).
+// launches are most of the time (a plan's clip of 65 pieces 11.6 -> 8.3 us, of 576 12.0 -> 9.2, of 1024 12.2 -> 11.3, of 1152
+// 13.6 -> 13.5, of 2304 20.2 -> 23.1 us: every workgroup's microsecond adds up).
 template <int NORM, typename Source>
 __global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const Source src, const int64_t n_parts, float* total, float max_norm,
                                                                  float scale, const float* scale_dev, const Partials partials)

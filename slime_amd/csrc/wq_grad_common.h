@@ -217,9 +217,10 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm, fl
 }
 
 // workspace: 64 bytes of AdamW's per-step values, one partial per piece, and the sums of kFoldGroup partials each that long
-// lists fold first (norms of 12 300 pieces 33.9 us in one fold, 35.8 in two; of 27 600 68.5 and 68.9; of 55 300 130.4 and 127.9).
+// lists fold first (norms of 17 280 pieces 44.8 us in one fold, 45.9 in two; of 27 648 68.2 and 68.6; of 32 640 79.2 and 79.3; of 36 864
+// 88.4 and 88.1; of 55 296 130.4 and 127.9; of 110 592 260 and 247).
 constexpr int64_t kGradControlBytes = 64;
-constexpr int64_t kFoldGroup = 4096, kFoldDirect = 4 * kFoldGroup;
+constexpr int64_t kFoldGroup = 4096, kFoldDirect = 8 * kFoldGroup;
 inline char* partials_of(void* workspace) { return (char*)workspace + kGradControlBytes; }
 struct Partials {
     const char* at;

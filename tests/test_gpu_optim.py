@@ -816,3 +816,97 @@ def test_workspaces_of_sixteen_byte_alignment(cuda):
     assert lib.wq_grad_norm_items(other._items.data_ptr(), other._n_items, 8, None, 0, 0, 0.25, None, room.data_ptr() + 16, total.data_ptr(),
                                   None, st) == 0
     assert torch.equal(total, plan.total_norm) and room[0].item() == 0 and room[1].item() == 0
+
+
+# ---- lists whose partials are folded in two levels ----------------------------------------------------------------------------
+FOLD_GROUP, FOLD_DIRECT = 4096, 8 * 4096
+
+
+@pytest.fixture(autouse=True)
+def seeded(request):
+    """What a test draws on the device is the same on each run of it."""
+    import zlib
+
+    torch.manual_seed(zlib.crc32(request.node.name.encode()))
+
+
+def long_list(pieces, dtype, device):
+    """Tensors of so many pieces in all, the first one nearly all of them; non-zero everywhere."""
+    item = ITEM // torch.empty((), dtype=dtype).element_size()
+    buf = torch.empty(pieces * item, dtype=dtype, device=device).normal_()
+    buf[buf == 0] = 1
+    cuts = [0, (pieces - 41) * item] + [(pieces - 40 + i) * item for i in range(41)]
+    return buf, [buf[a:b] for a, b in zip(cuts, cuts[1:])]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("pieces", [FOLD_DIRECT, FOLD_DIRECT + 1, FOLD_DIRECT + 3 * FOLD_GROUP + 1000])
+def test_long_norms(cuda, pieces, dtype):
+    buf, ts = long_list(pieces, dtype, cuda)
+    plans = {k: slime_amd.GradNormPlan(ts, k, per_tensor=True) for k in (2.0, math.inf)}
+    assert plans[2.0]._n_items == pieces
+    for k, plan in plans.items():
+        total, each = plan.run()
+        check_norm(total, ts, k)
+        check_norm(slime_amd.get_total_norm(ts, k), ts, k)
+        check_norm(plan.run(grad_scale=0.37)[0], ts, k, float(torch.tensor(0.37)))
+        plan.run()
+        for e, t in zip(each, ts):
+            check_norm(e, [t], k)
+    # every group of partials counts: a value that stands out in each in turn, at the first and the last place of it
+    item, groups = buf.numel() // pieces, -(-pieces // FOLD_GROUP)
+    rest = norm_of([buf])
+    for group in range(groups):
+        for at in (group * FOLD_GROUP * item, min((group + 1) * FOLD_GROUP, pieces) * item - 1):
+            old = buf[at].clone()
+            buf[at] = 65536.0
+            want = math.sqrt(rest ** 2 - old.double().item() ** 2 + 2.0 ** 32)
+            assert plans[math.inf].run()[0].item() == 65536.0 == slime_amd.get_total_norm(ts, math.inf).item()
+            assert abs(plans[2.0].run()[0].item() - want) <= 2 * U * want
+            buf[at] = math.nan
+            assert all(math.isnan(p.run()[0].item()) for p in plans.values())
+            buf[at] = old
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_long_clips(cuda, norm_type, dtype):
+    buf, ts = long_list(FOLD_DIRECT + 2 * FOLD_GROUP + 77, dtype, cuda)
+    before = buf.clone()
+    norm = norm_of([before], norm_type)
+    check_norm(slime_amd.GradClipPlan(ts, norm_type).run(0.3 * norm), [before], norm_type)
+    check_clip([buf], [before], 0.3 * norm, norm)
+    buf.copy_(before)
+    ps = [torch.nn.Parameter(t.new_empty(t.shape)) for t in ts]
+    for p, t in zip(ps, ts):
+        p.grad = t
+    check_norm(slime_amd.clip_grad_norm_(ps, 0.3 * norm, norm_type), [before], norm_type)
+    check_clip([buf], [before], 0.3 * norm, norm)
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+@pytest.mark.parametrize("pieces", [FOLD_DIRECT, FOLD_DIRECT + FOLD_GROUP + 5])
+def test_long_updates(cuda, norm_type, pieces):
+    """The folded sums feed the step's scalars; on both sides of the limit for plain loads, too."""
+    n = pieces * _lib.ADAMW_ITEM
+    g = torch.empty(n, dtype=BF16, device=cuda).normal_()
+    p, m, v = (torch.zeros(n, device=cuda) for _ in range(3))
+    cut = n - 3 * _lib.ADAMW_ITEM
+    plan = slime_amd.AdamWPlan(*([x[:cut], x[cut:]] for x in (p, g)), exp_avgs=[m[:cut], m[cut:]], exp_avg_sqs=[v[:cut], v[cut:]],
+                               norm_type=norm_type, skip_nonfinite=True, weight_decay=0.0)
+    assert plan._n_items == pieces
+    norm = norm_of([g], norm_type)
+    check_norm(plan.run(1e-2, max_norm=0.5 * norm), [g], norm_type)
+    c = 0.5 * norm / (norm + 1e-6)
+    for a in range(0, n, 1 << 25):
+        s = slice(a, min(a + (1 << 25), n))
+        zero = torch.zeros(s.stop - a, device=cuda)
+        want = adamw_bounds(g[s], zero, zero, zero, 1, c, 1e-2, 1.0, 0.0, 0.9, 0.999, 1e-8, 5)
+        for x, (val, bound) in zip((p[s], m[s], v[s]), want):
+            near(x, val, bound)
+    old = p.clone()
+    for at in (5, FOLD_GROUP * _lib.ADAMW_ITEM * 4 + 1, n - 1):           # a NaN in any group stops the step
+        keep = g[at].clone()
+        g[at] = math.nan
+        assert math.isnan(plan.run(1e-2).item()) and plan.step.item() == 1 and torch.equal(p, old)
+        g[at] = keep
