@@ -158,7 +158,8 @@ template <> struct NormAcc<WQ_NORM_INF> {
     static __device__ __forceinline__ T zero() { return 0; }
     static __device__ __forceinline__ T join(T a, T b) { return a > b ? a : b; }
     static __device__ __forceinline__ void add(T& a, float x) { a = (uint64_t)max((uint32_t)a, f2u(x) & 0x7FFFFFFFu); }
-    static __device__ __forceinline__ float finish(T a, float scale) { return u2f((uint32_t)a) * __builtin_fabsf(scale); }
+    // without a sign, also where infinity times 0 makes a NaN (with a sign, here): bits order like norms
+    static __device__ __forceinline__ float finish(T a, float scale) { return __builtin_fabsf(u2f((uint32_t)a) * scale); }
 };
 
 template <typename T>

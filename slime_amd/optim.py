@@ -10,8 +10,10 @@ whatever gradients a call presents; ``GradNormPlan``, ``GradClipPlan`` and ``Ada
 stay where they are) and can be captured into a HIP graph.  Norms are fp32, whatever the gradients' type: sums of squares are
 formed in 64 bits in a fixed order, so they neither overflow nor depend on the run (a norm beyond fp32's range is infinite).
 
-Norm of a model that is sharded over ranks: ``norm = plan.run(); total = norm.square(); all_reduce(total);`` and
-``total_norm=total.sqrt()`` in the clip or the update.
+Norm of a model that is sharded over ranks, for ``total_norm=`` of the clip or the update: of 2-norms
+``total = plan.run().double().square(); all_reduce(total); total_norm = total.sqrt().float()`` (fp32 squares would be infinite for a
+norm above 1.8e19 and zero below 2.6e-23); of infinity norms ``total_norm = plan.run(); all_reduce(total_norm.view(torch.int32),
+op=MAX)`` (the bits of magnitudes have their order, and a NaN on one rank is above infinity; of floats a maximum may drop it).
 """
 
 from __future__ import annotations

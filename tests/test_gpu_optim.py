@@ -910,3 +910,45 @@ def test_long_updates(cuda, norm_type, pieces):
         g[at] = math.nan
         assert math.isnan(plan.run(1e-2).item()) and plan.step.item() == 1 and torch.equal(p, old)
         g[at] = keep
+
+
+# ---- norms over ranks ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [1.0, 1e23, 1e-28])
+def test_norms_of_parts_reduced_as_over_ranks(cuda, scale):
+    """Two lists stand for two ranks' parts; the reductions are those that the module gives, without the collective."""
+    parts = [tensors(SIZES, [F32], 120 + i, scale) for i in range(2)]
+    both = parts[0] + parts[1]
+    before = [[t.clone() for t in ts] for ts in parts]
+    squares = [slime_amd.GradNormPlan(ts).run().double().square() for ts in parts]
+    total = (squares[0] + squares[1]).sqrt().float()
+    want = norm_of(both)
+    assert abs(total.item() - want) <= 3 * U * want                         # each part's rounding, and the last one
+    for ts, old in zip(parts, before):
+        slime_amd.GradClipPlan(ts).run(0.25 * want, total_norm=total)
+        c = 0.25 * want / (want + 1e-6)
+        for t, o in zip(ts, old):                                          # a coefficient's 6 u, and 2 more of the norm
+            assert bool(((t.double() - o.double() * c).abs() <= o.double().abs() * c * 8.01 * U + SUBNORMAL[F32]).all())
+    biggest = [slime_amd.GradNormPlan(ts, math.inf).run() for ts in before]
+    largest = torch.maximum(*(b.view(torch.int32) for b in biggest)).view(F32)
+    check_norm(largest, before[0] + before[1], math.inf)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_the_bits_of_an_infinity_norm_order_like_it(cuda, dtype):
+    """NaN above infinity above the rest, as integers: whatever the sign and payload of the NaN, and for infinity times 0."""
+    x = torch.zeros(100, dtype=dtype, device=cuda)
+    plan = slime_amd.GradNormPlan([x], math.inf)
+    inf = int(torch.tensor(math.inf).view(torch.int32))
+    for bad in (math.nan, -math.nan):
+        x[3] = bad
+        for scale in (1.0, 0.5, torch.tensor(-2.0, device=cuda)):
+            assert plan.run(scale).view(torch.int32).item() > inf
+    if dtype == F32:
+        for bits in (0x7F800001, -1, -0x7FFFFF, 0x7FFFFFFF):
+            x.view(torch.int32)[3] = bits
+            assert plan.run().view(torch.int32).item() > inf and plan.run(0.5).view(torch.int32).item() > inf
+    x[3] = -math.inf
+    assert plan.run().view(torch.int32).item() == inf
+    assert plan.run(0.0).view(torch.int32).item() > inf
+    x[3] = 1.0
+    assert 0 < plan.run().view(torch.int32).item() < inf

@@ -575,3 +575,38 @@ def test_numbers_that_fp32_cannot_hold_are_refused(host_plans):
     optim.AdamWPlan(_lists(), _lists(), eps=1e-45).run(most)
     optim.AdamWPlan(_lists(), _lists(), eps=0.0, weight_decay=most, lr_scale=most)
     assert _lib.load().wq_adamw_items(None, 1, _hyper(eps=1e-45), P, None) == N_
+
+
+# ---- norms over ranks ---------------------------------------------------------------------------------------------------------
+RANK_NORMS = [(3.0, 4.0), (1e25, 3e25), (1e-30, 2e-30), (0.0, 0.0), (math.inf, 1.0), (1.0, math.nan), (math.nan, math.inf), (3e38, 3e38)]
+
+
+def _reduce_on_rank(rank, port, results):
+    import torch.distributed as dist
+
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2)
+    for i, norms in enumerate(RANK_NORMS):
+        norm = torch.tensor(norms[rank])                 # as a plan on this rank returns it
+        total = norm.double().square()
+        dist.all_reduce(total)
+        results[i, rank, 0] = total.sqrt().float()
+        dist.all_reduce(norm.view(torch.int32), op=dist.ReduceOp.MAX)
+        results[i, rank, 1] = norm
+    dist.destroy_process_group()
+
+
+def test_norms_over_ranks():
+    """The two reductions that the module gives, over two processes."""
+    import socket
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    results = torch.zeros(len(RANK_NORMS), 2, 2).share_memory_()
+    torch.multiprocessing.spawn(_reduce_on_rank, (port, results), nprocs=2)
+    for (a, b), got in zip(RANK_NORMS, results):
+        a, b = (float(torch.tensor(x)) for x in (a, b))
+        nan = math.isnan(a) or math.isnan(b)
+        two = math.nan if nan else math.inf if math.inf in (a, b) else math.hypot(a, b)
+        want = torch.tensor([two, math.nan if nan else max(a, b)], dtype=torch.float64).float()
+        assert all(torch.equal(g.nan_to_num(-1.0, posinf=math.inf), want.nan_to_num(-1.0, posinf=math.inf)) for g in got), (a, b, got, want)
