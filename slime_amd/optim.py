@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import math
 import numbers
+import operator
 from array import array
 from bisect import bisect_left
 from contextlib import nullcontext
@@ -36,7 +37,7 @@ _NORMS = {2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 # Lists of hundreds of tensors are looked at by passes that stay in C, map() over these (40 ns a tensor); only where something is
 # out of the ordinary are they looked at one by one.
 _data_ptr, _numel, _is_contiguous, _get_device, _is_neg = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device", "is_neg"))
-_dtype, _layout, _shape, _nbytes = (getattr(torch.Tensor, n).__get__ for n in ("dtype", "layout", "shape", "nbytes"))
+_dtype, _layout, _shape, _nbytes, _grad = (getattr(torch.Tensor, n).__get__ for n in ("dtype", "layout", "shape", "nbytes", "grad"))
 _PLAIN_TYPES = {torch.Tensor, torch.nn.Parameter}
 _F32_MAX = float(np.finfo(np.float32).max)      # what the kernels take as fp32 has to be finite there
 
@@ -419,7 +420,9 @@ class AdamWPlan(_Plan):
 
     ``run(lr, max_norm=None, grad_scale=1.0, total_norm=None)``: lr is a number or one fp32 value on the device (a number is
     fixed in a captured run).  Parameters with other betas are a plan of their own; the norm over several plans comes from one
-    ``GradNormPlan`` as their ``total_norm``.  Returns the gradient norm before the clip where it is needed (max_norm or skip_nonfinite; a 0-d
+    ``GradNormPlan`` as their ``total_norm``.  The gradients are read where they were when the plan was built; if they were the
+    parameters' ``.grad`` and a parameter has another one now (``zero_grad()`` drops them unless ``set_to_none=False``), the run is
+    refused.  Returns the gradient norm before the clip where it is needed (max_norm or skip_nonfinite; a 0-d
     fp32 tensor that the next run overwrites, or the ``total_norm`` given), else None."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], weights: Sequence | None = None,
@@ -476,11 +479,21 @@ class AdamWPlan(_Plan):
         self.skip_nonfinite = bool(skip_nonfinite)
         self.step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._owned += [self.step, *fresh]
+        leaves = [p for p, g in zip(self.params, self.grads) if p.is_leaf and p.grad is not None and p.grad.data_ptr() == g.data_ptr()]
+        self._leaves = leaves, [p.grad for p in leaves]
         self._hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, 0.0, None, None, None, self.total_norm.data_ptr(),
                                       self.step.data_ptr(), 1.0, -1.0, self._norm, self.skip_nonfinite)
         self._built()
 
+    def _refuse_moved_grads(self) -> None:
+        for p, g in zip(*self._leaves):
+            if p.grad is not None and p.grad.data_ptr() != g.data_ptr():
+                raise RuntimeError(f"AdamWPlan: a parameter of shape {tuple(p.shape)} has another gradient tensor than the plan was built over; "
+                                   "keep gradients in place (zero_grad(set_to_none=False)) or build a new plan")
+
     def run(self, lr, max_norm: float | None = None, grad_scale=1.0, total_norm: torch.Tensor | None = None):
+        if any(map(operator.is_not, map(_grad, self._leaves[0]), self._leaves[1])):
+            self._refuse_moved_grads()
         max_norm = -1.0 if max_norm is None else _check_max_norm(max_norm, "AdamWPlan")
         h = self._hyper
         h.lr, h.lr_dev = self._factor(lr, "lr")

@@ -610,3 +610,30 @@ def test_norms_over_ranks():
         two = math.nan if nan else math.inf if math.inf in (a, b) else math.hypot(a, b)
         want = torch.tensor([two, math.nan if nan else max(a, b)], dtype=torch.float64).float()
         assert all(torch.equal(g.nan_to_num(-1.0, posinf=math.inf), want.nan_to_num(-1.0, posinf=math.inf)) for g in got), (a, b, got, want)
+
+
+def test_updates_refuse_gradients_that_moved(host_plans):
+    """zero_grad() drops the gradients by default: the plan kept the old ones and stepped on them without an error."""
+    ps = _params(_lists())
+    plan = optim.AdamWPlan(ps, [p.grad for p in ps])
+    views = optim.AdamWPlan(ps, [p.grad.detach() for p in ps])
+    apart = optim.AdamWPlan(ps, _lists())
+    plan.run(0.1), views.run(0.1), apart.run(0.1)
+    opt = torch.optim.SGD(ps, lr=0.0)
+    opt.zero_grad(set_to_none=False)
+    sum((p * 2).sum() for p in ps).backward()               # accumulates in place
+    plan.run(0.1), views.run(0.1), apart.run(0.1)
+    opt.zero_grad()
+    plan.run(0.1), views.run(0.1), apart.run(0.1)           # no gradient of its own: whoever drops it may fill the plan's
+    assert len(host_plans) == 9
+    sum((p * 2).sum() for p in ps[1:]).backward()
+    for p in (plan, views):
+        with pytest.raises(RuntimeError, match="another gradient tensor"):
+            p.run(0.1)
+    apart.run(0.1)
+    assert len(host_plans) == 10
+    fresh = optim.AdamWPlan(ps[1:], [p.grad for p in ps[1:]])
+    fresh.run(0.1)
+    y = torch.zeros(4, requires_grad=True) * 1.0            # not a leaf: has no gradient to compare with, and no warning
+    optim.AdamWPlan([y], [torch.zeros(4)]).run(0.1)
+    assert len(host_plans) == 12
