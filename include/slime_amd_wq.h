@@ -478,11 +478,13 @@ int wq_xxh3_128_grouped(const wq_xxh3_desc *descs, const int64_t *item_start, in
  * launches read one descriptor per piece - WQ_GRAD_ITEM_BYTES of a gradient, WQ_ADAMW_ITEM elements of a parameter - made from
  * per-tensor descriptors on the device by wq_grad_make_items.  The *_list forms take HOST arrays of the tensors' addresses,
  * element counts and types instead (read before the call returns) and pass them on in the kernel arguments,
- * WQ_GRAD_LIST_LAUNCH tensors a launch: no table to build, upload or keep, any number of tensors.  Sums of squares are formed in 64 bits and added in a fixed order: results do not change from call to
- * call and neither overflow nor lose small gradients (fp32 squares exactly).
+ * WQ_GRAD_LIST_LAUNCH tensors a launch: no table to build, upload or keep, any number of tensors.  Sums of squares are
+ * formed in 64 bits (fp32 squares exactly: nothing overflows or is lost) and added in a fixed order: the same call on the same
+ * addresses gives the same bits.
  *
  * grad_scale (an inverse loss scale, 1 / number of tokens ...) multiplies every gradient; if grad_scale_dev is not NULL the
- * factor is grad_scale * grad_scale_dev[0], read on the device.  A norm is that of the scaled gradients.
+ * factor is grad_scale * grad_scale_dev[0], read on the device.  A norm is that of the scaled gradients.  grad_scale_dev and
+ * total_given must not lie in memory that the norm or the clip writes (an update has read them and lr_dev before it writes).
  * coefficient = grad_scale * min(1, max_norm / (norm + 1e-6)), in fp32; a NaN norm makes it NaN, an infinite one 0 (NaN for
  * infinite max_norm), as torch.nn.utils.clip_grads_with_norm_ has it. */
 #define WQ_GRAD_ITEM_BYTES 16384

@@ -4,7 +4,8 @@
 //
 // Both are bound by HBM: the norm reads every gradient once, the clip reads it again and writes it.  One workgroup takes one
 // piece - 16 KiB of one tensor, in the table of an update the gradients of 8192 elements - and leaves one 64-bit partial; a fold of
-// the partials in a fixed order gives the norm (no atomics, so the same gradients give the same bits).  Squares are added in 64 bits: fp32 squares are
+// the partials in a fixed order gives the norm (no atomics: the same list at the same addresses gives the same bits; pieces end at
+// 128-byte lines, so other starts add in another order).  Squares are added in 64 bits: fp32 squares are
 // exact there and can neither overflow nor vanish.
 
 #include "wq_grad_common.h"
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(256) void grad_make_items_kernel(const int64_t* des
 
 // A norm whose gradients are read again right away (`again`) leaves them in the 256 MB Infinity Cache if they fit: plain
 // instead of non-temporal loads make the norm alone slower (202 MB of bf16: 35 -> 38 us) and norm and clip together faster
-// (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 83 -> 80 us); with 2.4 GB nothing is left to find (1060 -> 1087 us).
+// (174 MB of bf16 into fp32: 119 -> 106 us, 202 MB in place 83 -> 80 us); beyond it little is left to find (fp32 in place, 336 MB
+// 152.8 -> 150.4, 403 MB 181.4 -> 180.4) and then nothing (2.4 GB 1060 -> 1087 us).
 // The host knows the number of pieces only: a list of more small tensors than that is taken for a long one.
 constexpr int64_t kKeepPieces = (256 << 20) / WQ_GRAD_ITEM_BYTES;
 // The same for an update, whose pieces are 32 KiB of fp32 or 16 KiB of bf16 gradients and which comes back to a gradient while

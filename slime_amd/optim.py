@@ -8,7 +8,8 @@ the clip as a factor (no pass of its own) and writes the bf16 / fp16 weight that
 ``get_total_norm``, ``clip_grad_norm_`` and ``clip_grads_with_norm_`` have the names and arguments of ``torch.nn.utils`` and take
 whatever gradients a call presents; ``GradNormPlan``, ``GradClipPlan`` and ``AdamWPlan`` take a fixed list (gradient buffers that
 stay where they are) and can be captured into a HIP graph.  Norms are fp32, whatever the gradients' type: sums of squares are
-formed in 64 bits in a fixed order, so they neither overflow nor depend on the run (a norm beyond fp32's range is infinite).
+formed in 64 bits, so they do not overflow (a norm beyond fp32's range is infinite), and in an order that depends on the list, on where
+its tensors start and on the kind of call or plan, but not on the run.
 
 Norm of a model that is sharded over ranks, for ``total_norm=`` of the clip or the update: of 2-norms
 ``total = plan.run().double().square(); all_reduce(total); total_norm = total.sqrt().float()`` (fp32 squares would be infinite for a
@@ -273,7 +274,8 @@ def _item_table(rows: np.ndarray, device, what: str):
 class _Plan:
     """Tables and workspace of a fixed list.  One plan's runs - captured ones too - must be ordered on one stream (or by
     events): they share the workspace and the result.  The stream need not be the one the plan was built on.  The plan reads
-    and writes the tensors it was given, wherever their contents come from; one that moves needs a new plan."""
+    and writes the tensors it was given, wherever their contents come from; one that moves needs a new plan.  A graph that
+    captured a run needs the plan for as long as it is replayed."""
 
     # Tensors that a run writes while others of its workgroups may still read the run's device scalars (an AdamW run has read its
     # scalars before it writes any).
@@ -395,6 +397,10 @@ class GradClipPlan(_Plan):
         return self.total_norm if total_norm is None else total_norm
 
 
+def _address(t):
+    return t.data_ptr() if t.layout == torch.strided else None
+
+
 def _per_tensor(value, n: int, what: str):
     values = [float(value)] * n if isinstance(value, numbers.Real) else [float(v) for v in value]
     if len(values) != n:
@@ -479,7 +485,7 @@ class AdamWPlan(_Plan):
         self.skip_nonfinite = bool(skip_nonfinite)
         self.step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._owned += [self.step, *fresh]
-        leaves = [p for p, g in zip(self.params, self.grads) if p.is_leaf and p.grad is not None and p.grad.data_ptr() == g.data_ptr()]
+        leaves = [p for p, g in zip(self.params, self.grads) if p.is_leaf and p.grad is not None and _address(p.grad) == g.data_ptr()]
         self._leaves = leaves, [p.grad for p in leaves]
         self._hyper = _lib.AdamWHyper(self.betas[0], self.betas[1], self.eps, 0.0, None, None, None, self.total_norm.data_ptr(),
                                       self.step.data_ptr(), 1.0, -1.0, self._norm, self.skip_nonfinite)
@@ -487,7 +493,7 @@ class AdamWPlan(_Plan):
 
     def _refuse_moved_grads(self) -> None:
         for p, g in zip(*self._leaves):
-            if p.grad is not None and p.grad.data_ptr() != g.data_ptr():
+            if p.grad is not None and _address(p.grad) != g.data_ptr():
                 raise RuntimeError(f"AdamWPlan: a parameter of shape {tuple(p.shape)} has another gradient tensor than the plan was built over; "
                                    "keep gradients in place (zero_grad(set_to_none=False)) or build a new plan")
 
@@ -519,8 +525,9 @@ _SHARED = "gradients share memory (the same tensor twice?); they cannot be clipp
 
 class _List:
     """Tensors as the list entry points take them: host arrays of addresses, element counts and types.  The common case -
-    contiguous tensors of one GPU - is found out by passes that stay in C (0.2 us a tensor); anything else is looked at
-    one by one, for the message or for the copies that other strides need."""
+    contiguous tensors of one GPU - is found out by passes that stay in C (0.2 us a tensor; with the gathering of gradients, the
+    check for shared memory and the version counters of a clip 0.35); anything else is looked at one by one, for the message or
+    for the copies that other strides need."""
 
     def __init__(self, tensors, what: str, written: bool):
         self.copies, given = [], tensors

@@ -634,6 +634,12 @@ def test_updates_refuse_gradients_that_moved(host_plans):
     assert len(host_plans) == 10
     fresh = optim.AdamWPlan(ps[1:], [p.grad for p in ps[1:]])
     fresh.run(0.1)
+    table = torch.nn.Parameter(torch.zeros(4, 8))
+    table.grad = torch.zeros(4, 8).to_sparse()              # its dense sum is elsewhere
+    optim.AdamWPlan([table], [torch.zeros(4, 8)]).run(0.1)
     y = torch.zeros(4, requires_grad=True) * 1.0            # not a leaf: has no gradient to compare with, and no warning
     optim.AdamWPlan([y], [torch.zeros(4)]).run(0.1)
-    assert len(host_plans) == 12
+    assert len(host_plans) == 13
+    ps[0].grad = torch.zeros(4, 8).to_sparse()
+    with pytest.raises(RuntimeError, match="another gradient tensor"):
+        plan.run(0.1)
